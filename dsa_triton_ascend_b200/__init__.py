@@ -6,7 +6,9 @@ Public API = the operators of WhFanatic/dsa_triton_ascend with unchanged signatu
 `SparseFlashAttentionGradTriton` and the indexer's KL-loss backward
 `sparse_lightning_indexer_grad_kl_loss_triton` / `SparseLightningIndexerGradKLLossTriton`, and the
 dense counterpart with its statistics helper (`dense_loss_backward_triton`,
-`dense_lightning_indexer_softmax_lse_triton`, ... in `dense_loss_backward`).  All are thin wrappers over the C-ABI CUDA library built from
+`dense_lightning_indexer_softmax_lse_triton`, ... in `dense_loss_backward`).  Beside them, without a counterpart there,
+what a program needs around the latent paged cache: `rotary_embedding` / `rotary_embedding_grad` and
+`latent_cache_append`.  All are thin wrappers over the C-ABI CUDA library built from
 `dsa_triton_ascend_b200/csrc` (declared in `include/dsa_b200.h`).  `check_status()` (an
 addition) reports a device-side wait that ran out in the latest call of either operator.
 """
@@ -23,6 +25,8 @@ from .dense_loss_backward import (DenseLightningIndexerGradKLLossTriton,  # noqa
                                   dense_lightning_indexer_softmax_lse_triton, dense_loss_backward_triton,
                                   npu_dense_lightning_indexer_grad_kl_loss_triton,
                                   npu_dense_lightning_indexer_softmax_lse_triton)
+from .rotary_embedding import RotaryEmbedding, rotary_embedding, rotary_embedding_grad  # noqa: F401
+from .latent_cache_append import LatentCacheAppend, latent_cache_append  # noqa: F401
 
 __all__ = [
     "lightning_indexer_triton", "LightningIndexerTriton",
@@ -33,5 +37,6 @@ __all__ = [
     "npu_dense_lightning_indexer_softmax_lse_triton", "dense_lightning_indexer_grad_kl_loss_triton",
     "npu_dense_lightning_indexer_grad_kl_loss_triton", "DenseLightningIndexerSoftmaxLseTriton",
     "DenseLossBackwardTriton", "DenseLightningIndexerGradKLLossTriton",
+    "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentCacheAppend",
     "check_status",
 ]

@@ -107,6 +107,36 @@ class DsaDenseLseParams(_c.Structure):
     ]
 
 
+class DsaRopeParams(_c.Structure):
+    _fields_ = [
+        ("struct_size", _c.c_uint32), ("inverse", _c.c_int32),
+        ("x", _c.c_void_p), ("positions", _c.c_void_p), ("inv_freq", _c.c_void_p), ("out", _c.c_void_p),
+        ("stride_b", _c.c_int64), ("stride_s", _c.c_int64), ("stride_n", _c.c_int64),
+        ("dtype", _c.c_int32), ("positions_64bit", _c.c_int32),
+        ("batch", _c.c_int32), ("s1", _c.c_int32), ("n", _c.c_int32), ("d", _c.c_int32),
+        ("pairs", _c.c_int32), ("offset", _c.c_int32), ("interleaved", _c.c_int32), ("axes", _c.c_int32),
+        ("sections", _c.c_int32 * 4),
+    ]
+
+
+class DsaAppendParams(_c.Structure):
+    _fields_ = [
+        ("struct_size", _c.c_uint32), ("dtype", _c.c_int32),
+        ("latent", _c.c_void_p), ("key_rope", _c.c_void_p), ("index_key", _c.c_void_p), ("norm_weight", _c.c_void_p),
+        ("positions", _c.c_void_p), ("inv_freq", _c.c_void_p),
+        ("seq_q", _c.c_void_p), ("seq_k", _c.c_void_p), ("block_table", _c.c_void_p),
+        ("latent_cache", _c.c_void_p), ("rope_cache", _c.c_void_p), ("index_cache", _c.c_void_p),
+        ("latent_stride_b", _c.c_int64), ("latent_stride_s", _c.c_int64),
+        ("rope_stride_b", _c.c_int64), ("rope_stride_s", _c.c_int64),
+        ("index_stride_b", _c.c_int64), ("index_stride_s", _c.c_int64),
+        ("layout_q", _c.c_int32), ("batch", _c.c_int32), ("s1", _c.c_int32), ("d", _c.c_int32), ("d_rope", _c.c_int32),
+        ("d_index", _c.c_int32), ("index_offset", _c.c_int32), ("block_size", _c.c_int32), ("max_blocks", _c.c_int32),
+        ("interleaved", _c.c_int32), ("index_interleaved", _c.c_int32), ("positions_64bit", _c.c_int32),
+        ("dtype_w", _c.c_int32), ("axes", _c.c_int32), ("sections", _c.c_int32 * 4), ("norm_eps", _c.c_float),
+        ("key_rows", _c.c_int64),
+    ]
+
+
 EXPORTS = (
     "dsa_abi_version", "dsa_status_string", "dsa_read_device_status",
     "dsa_li_workspace_bytes", "dsa_li_forward", "dsa_li_forward_zeros", "dsa_li_uses_tensor_path",
@@ -115,6 +145,7 @@ EXPORTS = (
     "dsa_kernel_launch_count", "dsa_sfa_grad_workspace_bytes", "dsa_sfa_grad", "dsa_sfa_grad_uses_tensor_path",
     "dsa_sfa_grad_workspace_bytes_uncut", "dsa_sli_grad_workspace_bytes_uncut",
     "dsa_sli_grad_workspace_bytes", "dsa_sli_grad", "dsa_dense_li_lse_workspace_bytes", "dsa_dense_li_lse",
+    "dsa_rope", "dsa_latent_append",
 )
 
 
@@ -154,6 +185,10 @@ def _load():
     lib.dsa_dense_li_lse_workspace_bytes.restype = _c.c_int
     lib.dsa_dense_li_lse.argtypes = [_c.POINTER(DsaDenseLseParams), _c.c_void_p, _c.c_size_t, _c.c_void_p]
     lib.dsa_dense_li_lse.restype = _c.c_int
+    lib.dsa_rope.argtypes = [_c.POINTER(DsaRopeParams), _c.c_void_p]
+    lib.dsa_rope.restype = _c.c_int
+    lib.dsa_latent_append.argtypes = [_c.POINTER(DsaAppendParams), _c.c_void_p]
+    lib.dsa_latent_append.restype = _c.c_int
     lib.dsa_li_forward_static.argtypes = [_c.POINTER(DsaLiParams), _c.c_void_p]
     lib.dsa_li_forward_static.restype = _c.c_int
     lib.dsa_li_static_scratch_bytes.restype = _c.c_size_t

@@ -27,6 +27,12 @@ def require_cuda(*tensors):
             raise RuntimeError("dsa_triton_ascend_b200 runs on CUDA tensors only (there is no CPU path)")
 
 
+def same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors are on {first.device} and {t.device}: one device is needed")
+
+
 @functools.lru_cache(maxsize=256)
 def _cached_lengths(values, device):
     """Device copy of a tuple of lengths.  An upload from pageable host memory first waits for the

@@ -11,6 +11,7 @@
 #include "li_score_simt.cuh"
 #include "li_score_sm100.cuh"
 #include "li_topk.cuh"
+#include "rope.cuh"
 #include "sfa_fwd_mma.cuh"
 #include "sfa_fwd_sm100.cuh"
 #include "sfa_bwd_simt.cuh"
@@ -579,6 +580,112 @@ static int dense_lse_launch(const DsaDenseLseParams* p, float* scratch, int32_t*
   return DSA_OK;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Rotary positions, append to the paged caches
+// ---------------------------------------------------------------------------------------------
+// Pairs per axis as running sums; entries past the last axis hold all pairs.
+static bool rope_ends(int32_t axes, const int32_t* sections, int32_t pairs, int32_t (&ends)[3]) {
+  if (axes < 1 || axes > 4) return false;
+  int64_t sum = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (i < axes) {
+      if (sections[i] < 0) return false;
+      sum += sections[i];
+    }
+    if (i < 3) ends[i] = i < axes - 1 ? (int32_t)std::min<int64_t>(sum, pairs) : pairs;
+  }
+  return sum == pairs;
+}
+
+static int rope_validate(const DsaRopeParams* p) {
+  if (p == nullptr) return DSA_ERR_NULL;
+  if (p->struct_size != sizeof(DsaRopeParams)) return DSA_ERR_STRUCT;
+  if (!p->x || !p->positions || !p->inv_freq || !p->out) return DSA_ERR_NULL;
+  if (p->dtype < DSA_DTYPE_BF16 || p->dtype > DSA_DTYPE_FP32) return DSA_ERR_VALUE;
+  if (p->batch < 0 || p->s1 < 0 || p->n < 0 || p->d < 2 || p->d > 1024) return DSA_ERR_VALUE;
+  if (p->pairs < 1 || p->offset < 0 || p->pairs > p->d / 2 || p->offset > p->d - 2 * p->pairs) return DSA_ERR_VALUE;
+  int32_t ends[3];
+  if (!rope_ends(p->axes, p->sections, p->pairs, ends)) return DSA_ERR_VALUE;
+  // (a block walks over its tokens' units in 32 bits)
+  if ((int64_t)p->n * p->d > (1 << 28)) return DSA_ERR_TOO_LARGE;
+  return DSA_OK;
+}
+
+template <typename T>
+static int rope_call(const DsaRopeParams* p, cudaStream_t st) {
+  RopeDev a;
+  a.x = p->x; a.out = p->out; a.positions = p->positions; a.inv_freq = p->inv_freq;
+  a.stride_b = p->stride_b; a.stride_s = p->stride_s; a.stride_n = p->stride_n;
+  a.tokens = (int64_t)p->batch * p->s1;
+  a.s1 = p->s1; a.n = p->n; a.d = p->d; a.pairs = p->pairs; a.offset = p->offset;
+  a.interleaved = p->interleaved != 0; a.pos64 = p->positions_64bit != 0;
+  rope_ends(p->axes, p->sections, p->pairs, a.ends);
+  a.sign = p->inverse ? -1.f : 1.f;
+  if (a.tokens == 0 || a.n == 0) return DSA_OK;
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool wide = !off16(p->x, p->out) && p->d % V == 0 && p->pairs % V == 0 && p->offset % V == 0 &&
+                    p->stride_b % V == 0 && p->stride_s % V == 0 && p->stride_n % V == 0;
+  return wide ? rope_launch<T, V>(a, st) : rope_launch<T, 1>(a, st);
+}
+
+static int append_validate(const DsaAppendParams* p) {
+  if (p == nullptr) return DSA_ERR_NULL;
+  if (p->struct_size != sizeof(DsaAppendParams)) return DSA_ERR_STRUCT;
+  if (!p->latent || !p->key_rope || !p->inv_freq || !p->seq_k || !p->block_table || !p->latent_cache || !p->rope_cache)
+    return DSA_ERR_NULL;
+  if ((p->index_key == nullptr) != (p->index_cache == nullptr)) return DSA_ERR_NULL;
+  if (p->dtype != DSA_DTYPE_BF16 && p->dtype != DSA_DTYPE_FP16) return DSA_ERR_VALUE;
+  if (p->norm_weight && p->dtype_w != p->dtype && p->dtype_w != DSA_DTYPE_FP32) return DSA_ERR_VALUE;
+  if (p->layout_q != DSA_LAYOUT_BSND && p->layout_q != DSA_LAYOUT_TND) return DSA_ERR_VALUE;
+  if (p->layout_q == DSA_LAYOUT_TND && !p->seq_q) return DSA_ERR_VALUE;
+  if (p->batch < 1 || p->s1 < 0 || p->block_size < 1 || p->max_blocks < 0 || p->key_rows < 0) return DSA_ERR_VALUE;
+  if (p->d != 128 && p->d != 256 && p->d != 512) return DSA_ERR_VALUE;
+  if (p->d_rope != 64) return DSA_ERR_VALUE;
+  if (p->index_key && (p->d_index < 64 || p->d_index > 1024 || p->d_index % 2 || p->index_offset < 0 || p->index_offset % 2 ||
+                       p->index_offset > p->d_index - 64))
+    return DSA_ERR_VALUE;
+  int32_t ends[3];
+  if (p->positions && !rope_ends(p->axes, p->sections, 32, ends)) return DSA_ERR_VALUE;
+  if ((int64_t)p->max_blocks * p->block_size > 0x7FFFFFFF) return DSA_ERR_TOO_LARGE;
+  if (p->layout_q == DSA_LAYOUT_BSND && (int64_t)p->batch * p->s1 > 0x7FFFFFFF) return DSA_ERR_TOO_LARGE;
+  // wide loads and stores: latents 16 bytes, pairs of the others 4
+  if (off16(p->latent, p->latent_cache) || off16(p->norm_weight) || p->latent_stride_b % 8 || p->latent_stride_s % 8)
+    return DSA_ERR_VALUE;
+  if ((((uintptr_t)p->key_rope | (uintptr_t)p->rope_cache | (uintptr_t)p->index_key | (uintptr_t)p->index_cache) & 3u) ||
+      p->rope_stride_b % 2 || p->rope_stride_s % 2 || p->index_stride_b % 2 || p->index_stride_s % 2)
+    return DSA_ERR_VALUE;
+  return DSA_OK;
+}
+
+template <typename T>
+static int append_call(const DsaAppendParams* p, cudaStream_t st) {
+  AppendDev a;
+  a.seq.seq_q = p->seq_q; a.seq.seq_k = p->seq_k; a.seq.block_table = p->block_table;
+  a.seq.layout_q = p->layout_q; a.seq.layout_k = DSA_LAYOUT_PA_BSND;
+  a.seq.seq_q_cum = p->layout_q == DSA_LAYOUT_TND; a.seq.seq_k_cum = 0;
+  a.seq.batch = p->batch; a.seq.s1 = p->s1; a.seq.s2 = p->max_blocks * p->block_size;
+  a.seq.block_size = p->block_size; a.seq.max_blocks = p->max_blocks; a.seq.sparse_mode = 0;
+  a.seq.key_rows = p->key_rows;
+  a.latent = p->latent; a.key_rope = p->key_rope; a.index_key = p->index_key; a.norm_weight = p->norm_weight;
+  a.positions = p->positions; a.inv_freq = p->inv_freq;
+  a.latent_cache = p->latent_cache; a.rope_cache = p->rope_cache; a.index_cache = p->index_cache;
+  a.latent_b = p->latent_stride_b; a.latent_s = p->latent_stride_s;
+  a.rope_b = p->rope_stride_b; a.rope_s = p->rope_stride_s;
+  a.index_b = p->index_stride_b; a.index_s = p->index_stride_s;
+  a.tokens = p->layout_q == DSA_LAYOUT_TND ? p->s1 : (int64_t)p->batch * p->s1;
+  a.d = p->d; a.d_index = p->d_index; a.index_offset = p->index_offset;
+  a.interleaved = p->interleaved; a.index_interleaved = p->index_interleaved;
+  a.pos64 = p->positions_64bit != 0; a.weight_fp32 = p->dtype_w == DSA_DTYPE_FP32;
+  a.ends[0] = a.ends[1] = a.ends[2] = 32;
+  if (p->positions) rope_ends(p->axes, p->sections, 32, a.ends);
+  a.eps = p->norm_eps;
+  if (a.tokens == 0 || p->max_blocks == 0 || p->key_rows == 0) return DSA_OK;
+  const dim3 grid((unsigned)((a.tokens + kAppendWarps - 1) / kAppendWarps));
+  if (launch_after(latent_append_kernel<T>, dim3(grid), dim3(kAppendWarps * 32), 0, st, a) != cudaSuccess) return DSA_ERR_CUDA;
+  count_launch();
+  return DSA_OK;
+}
+
 }  // namespace dsa
 
 using namespace dsa;
@@ -835,6 +942,25 @@ int dsa_li_forward_static(const DsaLiParams* p, void* stream) {
   float* scores = reinterpret_cast<float*>((char*)scratch + kWorkspaceHeader);
   if (p->dtype_qk == DSA_DTYPE_BF16) return li_launch<__nv_bfloat16>(p, scores, cs);
   return li_launch<__half>(p, scores, cs);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rotary positions, append to the paged caches
+// ---------------------------------------------------------------------------------------------
+int dsa_rope(const DsaRopeParams* p, void* stream) {
+  const int rc = rope_validate(p);
+  if (rc != DSA_OK) return rc;
+  cudaStream_t cs = (cudaStream_t)stream;
+  if (p->dtype == DSA_DTYPE_BF16) return rope_call<__nv_bfloat16>(p, cs);
+  if (p->dtype == DSA_DTYPE_FP16) return rope_call<__half>(p, cs);
+  return rope_call<float>(p, cs);
+}
+
+int dsa_latent_append(const DsaAppendParams* p, void* stream) {
+  const int rc = append_validate(p);
+  if (rc != DSA_OK) return rc;
+  cudaStream_t cs = (cudaStream_t)stream;
+  return p->dtype == DSA_DTYPE_BF16 ? append_call<__nv_bfloat16>(p, cs) : append_call<__half>(p, cs);
 }
 
 #ifdef DSA_TOPK_PROFILE

@@ -1,0 +1,123 @@
+"""Rotary positions of queries and keys on B200, with one position axis or several, and their gradient.
+
+No counterpart in the reference, whose operators take `query_rope`, `key_rope` and the index queries and keys already
+rotated (sparse_flash_attention_triton.py:1317-1339).  Names, layouts and checks follow the other operators.
+"""
+import ctypes
+
+import torch
+
+from . import _cabi
+from ._host import current_stream, device_guard, dtype_code, ptr, require_cuda, same_device
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+MAX_AXES = 4
+
+
+def section_sizes(axis_sections, pairs):
+    """(axes, pairs per axis) of `axis_sections`; None: one axis."""
+    if axis_sections is None:
+        return 1, (pairs,)
+    sections = tuple(int(n) for n in axis_sections)
+    if not 1 <= len(sections) <= MAX_AXES or min(sections) < 0 or sum(sections) != pairs:
+        raise ValueError(f"axis_sections must be 1 to {MAX_AXES} numbers of pairs whose sum is {pairs}, got {axis_sections}")
+    return len(sections), sections
+
+
+def check_positions(positions, tokens, axis_sections, what="positions"):
+    """`positions` of shape `tokens`, or [axes, *tokens] where axis_sections are given, as a contiguous tensor."""
+    want = tuple(tokens) if axis_sections is None else (len(axis_sections), *tokens)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what} must be int32 or int64, got {positions.dtype}")
+    if tuple(positions.shape) != want:
+        raise ValueError(f"{what} must have shape {want}, got {tuple(positions.shape)}")
+    return positions.contiguous()
+
+
+def check_inv_freq(inv_freq):
+    if inv_freq.dtype != torch.float32 or inv_freq.ndim != 1 or inv_freq.numel() < 1:
+        raise ValueError("inv_freq must be a float32 vector with an entry per pair")
+    return inv_freq.contiguous()
+
+
+def _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what):
+    if layout not in ("BSND", "TND"):
+        raise ValueError(f"layout must be BSND or TND, got {layout}")
+    if x.ndim != (4 if layout == "BSND" else 3):
+        raise ValueError(f"{what} must be {'[B,S,N,D]' if layout == 'BSND' else '[T,N,D]'}, got {tuple(x.shape)}")
+    code = dtype_code(x, _DTYPES, what)
+    inv_freq = check_inv_freq(inv_freq)
+    pairs, D = inv_freq.numel(), x.shape[-1]
+    if D > 1024 or rotary_offset < 0 or rotary_offset + 2 * pairs > D:
+        raise ValueError(f"{pairs} pairs from feature {rotary_offset} on do not fit {D} features (at most 1024)")
+    axes, sections = section_sizes(axis_sections, pairs)
+    positions = check_positions(positions, x.shape[:-2], axis_sections)
+    require_cuda(x, positions, inv_freq)
+    same_device(x, positions, inv_freq)
+    if x.stride(-1) != 1 and D > 1:
+        x = x.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    p = _cabi.DsaRopeParams()
+    p.struct_size = ctypes.sizeof(_cabi.DsaRopeParams)
+    p.inverse = 1 if inverse else 0
+    p.x, p.positions, p.inv_freq, p.out = ptr(x), ptr(positions), ptr(inv_freq), ptr(out)
+    p.stride_b = x.stride(0) if layout == "BSND" else 0
+    p.stride_s, p.stride_n = x.stride(-3), x.stride(-2)
+    p.dtype, p.positions_64bit = code, 1 if positions.dtype == torch.int64 else 0
+    p.batch, p.s1 = (x.shape[0], x.shape[1]) if layout == "BSND" else (1, x.shape[0])
+    p.n, p.d = x.shape[-2], D
+    p.pairs, p.offset, p.interleaved, p.axes = pairs, rotary_offset, 1 if interleaved else 0, axes
+    for i, n in enumerate(sections):
+        p.sections[i] = n
+    dev = x.device
+    with device_guard(dev):
+        _cabi.check(_cabi.lib.dsa_rope(ctypes.byref(p), current_stream(dev)), "rotary_embedding")
+    return out
+
+
+def rotary_embedding(x, positions, inv_freq, layout: str = "BSND", interleaved: bool = True, rotary_offset: int = 0,
+                     axis_sections=None):
+    """Rotate features of queries or keys by their tokens' positions.
+
+    Pair j of the rotated features, as one complex number, is multiplied by exp(i p inv_freq[j]).
+
+    Args:
+        x: [B,S,N,D] BSND or [T,N,D] TND, bf16 / fp16 / fp32, D up to 1024; any strides (a slice of a projection is read
+            in place as long as its last dimension is contiguous)
+        positions: int32 or int64 [B,S] / [T]; with axis_sections [axes,B,S] / [axes,T]
+        inv_freq: float32 [pairs], radians per position
+        interleaved: a pair is features (2j, 2j + 1) of the rotated ones; otherwise (j, j + pairs)
+        rotary_offset: first rotated feature; the 2 * pairs features from there on are rotated, the others copied
+        axis_sections: pairs per position axis (time, height, width, ...), in order, up to four axes; None: one axis
+
+    Returns: a new contiguous tensor of x's shape and dtype.  Angles are taken in 64 bits, sine, cosine and the rotation
+    in 32.  Nothing is recorded for autograd; the gradient is `rotary_embedding_grad`.
+    """
+    return _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, False, "x")
+
+
+def rotary_embedding_grad(d_out, positions, inv_freq, layout: str = "BSND", interleaved: bool = True,
+                          rotary_offset: int = 0, axis_sections=None):
+    """Gradient of `rotary_embedding` with respect to x, given the gradient of its result: the rotation by the
+    opposite angles.  Arguments as there; positions and frequencies are not differentiated."""
+    return _rotate(d_out, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, True, "d_out")
+
+
+class RotaryEmbedding(torch.nn.Module):
+    """Attribute holder around rotary_embedding."""
+
+    def __init__(self, inv_freq, layout="BSND", interleaved=True, rotary_offset=0, axis_sections=None):
+        super().__init__()
+        self.register_buffer("inv_freq", inv_freq, persistent=False)
+        self.layout = layout
+        self.interleaved = interleaved
+        self.rotary_offset = rotary_offset
+        self.axis_sections = axis_sections
+
+    def forward(self, x, positions):
+        return rotary_embedding(x, positions, self.inv_freq, self.layout, self.interleaved, self.rotary_offset,
+                                self.axis_sections)
+
+    construct = forward

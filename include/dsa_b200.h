@@ -314,6 +314,74 @@ int dsa_dense_li_lse(const DsaDenseLseParams* p, void* workspace, size_t workspa
 int dsa_li_forward_static(const DsaLiParams* p, void* stream);
 size_t dsa_li_static_scratch_bytes(void);
 
+/*
+ * Rotary positions (no counterpart in the reference, whose operators take query_rope, key_rope and the index queries and
+ * keys already rotated).  Pair j of the rotated features of a head is turned by the angle p * inv_freq[j]; with
+ * inverse = 1 by minus that angle, which is the gradient of the rotation.  p is the token's position on the pair's axis:
+ * the first sections[0] pairs follow positions[0], the next sections[1] positions[1], and so on (axes = 1: all of them).
+ * Rotated are the features offset .. offset + 2 * pairs - 1: neighbours (2j, 2j + 1) as a pair where interleaved,
+ * else (j, j + pairs); the others pass through.  out is contiguous, x has strides (in elements; its last dimension is
+ * contiguous) and may not overlap out.  No workspace.
+ */
+typedef struct DsaRopeParams {
+  uint32_t struct_size; /* sizeof(DsaRopeParams) */
+  int32_t inverse;
+  const void* x;         /* [batch, s1, n, d], dtype                          */
+  const void* positions; /* [axes, batch * s1], int32 or int64                */
+  const float* inv_freq; /* [pairs]                                           */
+  void* out;             /* [batch, s1, n, d], dtype, contiguous              */
+  int64_t stride_b, stride_s, stride_n;
+  int32_t dtype;         /* DSA_DTYPE_BF16 | FP16 | FP32                      */
+  int32_t positions_64bit;
+  int32_t batch, s1, n, d;               /* d <= 1024                         */
+  int32_t pairs, offset, interleaved;    /* offset + 2 * pairs <= d           */
+  int32_t axes;                          /* 1 .. 4                            */
+  int32_t sections[4];                   /* pairs per axis, their sum = pairs */
+} DsaRopeParams;
+int dsa_rope(const DsaRopeParams* p, void* stream);
+
+/*
+ * Append of new tokens to the paged caches that the indexer and the attention read (no counterpart in the reference):
+ * the latent (optionally normalised: x * rsqrt(mean(x^2) + norm_eps) * norm_weight), the rope key (rotated) and the index
+ * key (64 of its features rotated, by the same angles).  seq_q, seq_k and block_table are those of the attention
+ * call that follows: seq_k counts the new tokens, token i of a sequence goes to position seq_k - seq_q + i, through
+ * block_table.  That position is also the one that it is rotated by, unless `positions` names others.  Tokens past
+ * their sequence's query length, at positions before 0 or past the table, or whose block is absent (-1) or beyond the
+ * cache are left out; slots that no token goes to are left as they are.  No two tokens of a call may share a
+ * slot.  No workspace.
+ */
+typedef struct DsaAppendParams {
+  uint32_t struct_size; /* sizeof(DsaAppendParams) */
+  int32_t dtype;           /* DSA_DTYPE_BF16 | FP16 of tokens and caches                   */
+  const void* latent;      /* [batch, s1, 1, d] | [T1, 1, d], on 16-byte boundaries        */
+  const void* key_rope;    /* the same with 64, on 4-byte boundaries                       */
+  const void* index_key;   /* the same with d_index, on 4-byte boundaries; NULL: none      */
+  const void* norm_weight; /* [d], dtype_w, on a 16-byte boundary; NULL: no normalisation  */
+  const void* positions;   /* [axes, tokens], int32 or int64; NULL: position in the cache  */
+  const float* inv_freq;   /* [32] */
+  const int32_t* seq_q;    /* [batch] lengths or NULL; TND: cumulative ends                */
+  const int32_t* seq_k;    /* [batch] lengths */
+  const int32_t* block_table; /* [batch, max_blocks], -1 = no block                        */
+  void* latent_cache;      /* [blocks, block_size, 1, d]       */
+  void* rope_cache;        /* [blocks, block_size, 1, 64]      */
+  void* index_cache;       /* [blocks, block_size, 1, d_index] */
+  int64_t latent_stride_b, latent_stride_s; /* of a sequence (unused for TND) and of a token, in elements */
+  int64_t rope_stride_b, rope_stride_s;
+  int64_t index_stride_b, index_stride_s;
+  int32_t layout_q;        /* DSA_LAYOUT_BSND | DSA_LAYOUT_TND */
+  int32_t batch, s1;       /* TND: s1 = T1 */
+  int32_t d;               /* 128, 256 or 512 */
+  int32_t d_rope;          /* 64 */
+  int32_t d_index, index_offset; /* index_offset + 64 <= d_index, both even, d_index <= 1024 */
+  int32_t block_size, max_blocks;
+  int32_t interleaved, index_interleaved, positions_64bit, dtype_w;
+  int32_t axes;
+  int32_t sections[4];
+  float norm_eps;
+  int64_t key_rows;        /* blocks * block_size of the caches */
+} DsaAppendParams;
+int dsa_latent_append(const DsaAppendParams* p, void* stream);
+
 /* Static description of a status code. */
 const char* dsa_status_string(int status);
 /* Synchronises `stream` and returns the device status word stored at the start of a
