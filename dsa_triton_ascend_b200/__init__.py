@@ -7,8 +7,8 @@ Public API = the operators of WhFanatic/dsa_triton_ascend with unchanged signatu
 `sparse_lightning_indexer_grad_kl_loss_triton` / `SparseLightningIndexerGradKLLossTriton`, and the
 dense counterpart with its statistics helper (`dense_loss_backward_triton`,
 `dense_lightning_indexer_softmax_lse_triton`, ... in `dense_loss_backward`).  Beside them, without a counterpart there,
-what a program needs around the latent paged cache: `rotary_embedding` / `rotary_embedding_grad` and
-`latent_cache_append`.  All are thin wrappers over the C-ABI CUDA library built from
+what a program needs around the latent paged cache: `rotary_embedding` / `rotary_embedding_grad`,
+`latent_cache_append` and `shared_prefix_attention`.  All are thin wrappers over the C-ABI CUDA library built from
 `dsa_triton_ascend_b200/csrc` (declared in `include/dsa_b200.h`).  `check_status()` (an
 addition) reports a device-side wait that ran out in the latest call of either operator.
 """
@@ -25,8 +25,9 @@ from .dense_loss_backward import (DenseLightningIndexerGradKLLossTriton,  # noqa
                                   dense_lightning_indexer_softmax_lse_triton, dense_loss_backward_triton,
                                   npu_dense_lightning_indexer_grad_kl_loss_triton,
                                   npu_dense_lightning_indexer_softmax_lse_triton)
-from .rotary_embedding import RotaryEmbedding, rotary_embedding, rotary_embedding_grad  # noqa: F401
-from .latent_cache_append import LatentCacheAppend, latent_cache_append  # noqa: F401
+from .rotary import RotaryEmbedding, rotary_embedding, rotary_embedding_grad  # noqa: F401
+from .latent_cache import LatentCacheAppend, latent_cache_append  # noqa: F401
+from .prefix_attention import SharedPrefixAttention, shared_prefix_attention  # noqa: F401
 
 __all__ = [
     "lightning_indexer_triton", "LightningIndexerTriton",
@@ -38,5 +39,6 @@ __all__ = [
     "npu_dense_lightning_indexer_grad_kl_loss_triton", "DenseLightningIndexerSoftmaxLseTriton",
     "DenseLossBackwardTriton", "DenseLightningIndexerGradKLLossTriton",
     "rotary_embedding", "rotary_embedding_grad", "RotaryEmbedding", "latent_cache_append", "LatentCacheAppend",
+    "shared_prefix_attention", "SharedPrefixAttention",
     "check_status",
 ]

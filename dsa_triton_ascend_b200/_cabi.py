@@ -137,6 +137,19 @@ class DsaAppendParams(_c.Structure):
     ]
 
 
+class DsaSpaParams(_c.Structure):
+    _fields_ = [
+        ("struct_size", _c.c_uint32), ("kernel", _c.c_int32),
+        ("query", _c.c_void_p), ("query_rope", _c.c_void_p), ("key", _c.c_void_p), ("key_rope", _c.c_void_p),
+        ("seq_q", _c.c_void_p), ("seq_k", _c.c_void_p), ("block_table", _c.c_void_p), ("prefix_device", _c.c_void_p),
+        ("out", _c.c_void_p), ("softmax_max", _c.c_void_p), ("softmax_sum", _c.c_void_p),
+        ("layout_q", _c.c_int32), ("dtype", _c.c_int32), ("batch", _c.c_int32), ("s1", _c.c_int32),
+        ("n1", _c.c_int32), ("d", _c.c_int32), ("d_rope", _c.c_int32),
+        ("block_size", _c.c_int32), ("max_blocks", _c.c_int32), ("prefix", _c.c_int32),
+        ("sparse_mode", _c.c_int32), ("return_lse", _c.c_int32), ("scale", _c.c_float), ("key_rows", _c.c_int64),
+    ]
+
+
 EXPORTS = (
     "dsa_abi_version", "dsa_status_string", "dsa_read_device_status",
     "dsa_li_workspace_bytes", "dsa_li_forward", "dsa_li_forward_zeros", "dsa_li_uses_tensor_path",
@@ -145,7 +158,7 @@ EXPORTS = (
     "dsa_kernel_launch_count", "dsa_sfa_grad_workspace_bytes", "dsa_sfa_grad", "dsa_sfa_grad_uses_tensor_path",
     "dsa_sfa_grad_workspace_bytes_uncut", "dsa_sli_grad_workspace_bytes_uncut",
     "dsa_sli_grad_workspace_bytes", "dsa_sli_grad", "dsa_dense_li_lse_workspace_bytes", "dsa_dense_li_lse",
-    "dsa_rope", "dsa_latent_append",
+    "dsa_rope", "dsa_latent_append", "dsa_spa_workspace_bytes", "dsa_spa_forward", "dsa_spa_uses_tensor_path",
 )
 
 
@@ -189,6 +202,12 @@ def _load():
     lib.dsa_rope.restype = _c.c_int
     lib.dsa_latent_append.argtypes = [_c.POINTER(DsaAppendParams), _c.c_void_p]
     lib.dsa_latent_append.restype = _c.c_int
+    lib.dsa_spa_workspace_bytes.argtypes = [_c.POINTER(DsaSpaParams), _c.POINTER(_c.c_size_t)]
+    lib.dsa_spa_workspace_bytes.restype = _c.c_int
+    lib.dsa_spa_forward.argtypes = [_c.POINTER(DsaSpaParams), _c.c_void_p, _c.c_size_t, _c.c_void_p]
+    lib.dsa_spa_forward.restype = _c.c_int
+    lib.dsa_spa_uses_tensor_path.argtypes = [_c.POINTER(DsaSpaParams)]
+    lib.dsa_spa_uses_tensor_path.restype = _c.c_int
     lib.dsa_li_forward_static.argtypes = [_c.POINTER(DsaLiParams), _c.c_void_p]
     lib.dsa_li_forward_static.restype = _c.c_int
     lib.dsa_li_static_scratch_bytes.restype = _c.c_size_t

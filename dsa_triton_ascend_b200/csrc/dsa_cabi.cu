@@ -581,6 +581,73 @@ static int dense_lse_launch(const DsaDenseLseParams* p, float* scratch, int32_t*
 }
 
 // ---------------------------------------------------------------------------------------------
+// Attention over the paged latent cache behind a shared prefix
+// ---------------------------------------------------------------------------------------------
+static inline int64_t spa_rows(const DsaSpaParams* p) {
+  return p->layout_q == DSA_LAYOUT_TND ? (int64_t)p->s1 : (int64_t)p->batch * p->s1;
+}
+
+static int spa_validate(const DsaSpaParams* p) {
+  if (p == nullptr) return DSA_ERR_NULL;
+  if (p->struct_size != sizeof(DsaSpaParams)) return DSA_ERR_STRUCT;
+  if (!p->query || !p->query_rope || !p->key || !p->key_rope || !p->seq_k || !p->out) return DSA_ERR_NULL;
+  if (!p->block_table && p->max_blocks > 0) return DSA_ERR_NULL;
+  if ((p->softmax_max == nullptr) != (p->softmax_sum == nullptr)) return DSA_ERR_NULL;
+  if (p->return_lse && !p->softmax_max) return DSA_ERR_NULL;
+  if (p->layout_q != DSA_LAYOUT_BSND && p->layout_q != DSA_LAYOUT_TND) return DSA_ERR_VALUE;
+  if (p->layout_q == DSA_LAYOUT_TND && !p->seq_q) return DSA_ERR_NULL;
+  if (p->dtype != DSA_DTYPE_BF16 && p->dtype != DSA_DTYPE_FP16) return DSA_ERR_VALUE;
+  if (p->d != 512 || p->d_rope != 64) return DSA_ERR_VALUE;
+  if (p->batch < 1 || p->s1 < 0 || p->n1 < 1 || p->block_size < 1 || p->max_blocks < 0) return DSA_ERR_VALUE;
+  if (p->prefix < 0 || p->key_rows < 1) return DSA_ERR_VALUE;
+  if (p->sparse_mode != 0 && p->sparse_mode != 3) return DSA_ERR_VALUE;
+  if (p->kernel < DSA_KERNEL_AUTO || p->kernel > DSA_KERNEL_TENSOR) return DSA_ERR_VALUE;
+  if (off16(p->key, p->key_rope)) return DSA_ERR_VALUE;
+  // flat (token, head) rows and key positions are counted in 32 bits
+  if ((int64_t)p->max_blocks * p->block_size > 0x7FFFFFFF - 256 || spa_rows(p) * p->n1 > 0x7FFFFFFF - 256)
+    return DSA_ERR_TOO_LARGE;
+  return DSA_OK;
+}
+
+// The row-by-row form of the call: every visible key is a slot of the portable attention kernel.
+static SfaDev spa_dense_dev(const DsaSpaParams* p) {
+  SfaDev d = {};
+  d.seq.seq_q = p->seq_q; d.seq.seq_k = p->seq_k; d.seq.block_table = p->block_table;
+  d.seq.layout_q = p->layout_q; d.seq.layout_k = DSA_LAYOUT_PA_BSND;
+  d.seq.seq_q_cum = p->layout_q == DSA_LAYOUT_TND; d.seq.seq_k_cum = 0;
+  d.seq.batch = p->batch; d.seq.s1 = p->s1; d.seq.s2 = p->max_blocks * p->block_size;
+  d.seq.block_size = p->block_size; d.seq.max_blocks = p->max_blocks;
+  d.seq.sparse_mode = p->sparse_mode;
+  d.seq.key_rows = p->key_rows;
+  d.query = p->query; d.query_rope = p->query_rope; d.key = p->key; d.key_rope = p->key_rope;
+  d.out = p->out; d.softmax_max = p->softmax_max; d.softmax_sum = p->softmax_sum;
+  d.rows = (int32_t)spa_rows(p);
+  d.n1 = p->n1; d.d = p->d; d.d_rope = p->d_rope;
+  d.return_lse = p->return_lse != 0;
+  d.scale = p->scale;
+  return d;
+}
+
+template <typename T>
+static int spa_launch_dense(const DsaSpaParams* p, cudaStream_t st) {
+  const SfaDev d = spa_dense_dev(p);
+  const size_t stat_bytes = (size_t)d.rows * p->n1 * sizeof(float);
+  if (!p->return_lse && p->softmax_max &&
+      (cudaMemsetAsync(p->softmax_max, 0, stat_bytes, st) != cudaSuccess ||
+       cudaMemsetAsync(p->softmax_sum, 0, stat_bytes, st) != cudaSuccess))
+    return DSA_ERR_CUDA;
+  const size_t smem = (size_t)(kSfaSimtHeads + kSfaSimtKeys) * (p->d + p->d_rope + kSfaSimtPad) * sizeof(T);
+  if (cudaFuncSetAttribute(sfa_fwd_mma_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  const int32_t gy = (p->n1 + kSfaSimtHeads - 1) / kSfaSimtHeads;
+  if (gy > 65535) return DSA_ERR_TOO_LARGE;
+  sfa_fwd_mma_kernel<T, true><<<dim3((unsigned)d.rows, (unsigned)gy), kSfaSimtThreads, smem, st>>>(d);
+  if (cudaGetLastError() != cudaSuccess) return DSA_ERR_CUDA;
+  count_launch();
+  return DSA_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
 // Rotary positions, append to the paged caches
 // ---------------------------------------------------------------------------------------------
 // Pairs per axis as running sums; entries past the last axis hold all pairs.
@@ -631,7 +698,8 @@ static int rope_call(const DsaRopeParams* p, cudaStream_t st) {
 static int append_validate(const DsaAppendParams* p) {
   if (p == nullptr) return DSA_ERR_NULL;
   if (p->struct_size != sizeof(DsaAppendParams)) return DSA_ERR_STRUCT;
-  if (!p->latent || !p->key_rope || !p->inv_freq || !p->seq_k || !p->block_table || !p->latent_cache || !p->rope_cache)
+  if (!p->latent || !p->key_rope || !p->inv_freq || !p->seq_k || (!p->block_table && p->max_blocks > 0) ||
+      !p->latent_cache || !p->rope_cache)
     return DSA_ERR_NULL;
   if ((p->index_key == nullptr) != (p->index_cache == nullptr)) return DSA_ERR_NULL;
   if (p->dtype != DSA_DTYPE_BF16 && p->dtype != DSA_DTYPE_FP16) return DSA_ERR_VALUE;
@@ -942,6 +1010,32 @@ int dsa_li_forward_static(const DsaLiParams* p, void* stream) {
   float* scores = reinterpret_cast<float*>((char*)scratch + kWorkspaceHeader);
   if (p->dtype_qk == DSA_DTYPE_BF16) return li_launch<__nv_bfloat16>(p, scores, cs);
   return li_launch<__half>(p, scores, cs);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention over the paged latent cache behind a shared prefix
+// ---------------------------------------------------------------------------------------------
+int dsa_spa_uses_tensor_path(const DsaSpaParams* p) { return 0; }
+
+int dsa_spa_workspace_bytes(const DsaSpaParams* p, size_t* out_bytes) {
+  const int rc = spa_validate(p);
+  if (rc != DSA_OK) return rc;
+  if (!out_bytes) return DSA_ERR_NULL;
+  *out_bytes = kWorkspaceHeader;
+  return DSA_OK;
+}
+
+int dsa_spa_forward(const DsaSpaParams* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = spa_validate(p);
+  if (rc != DSA_OK) return rc;
+  size_t need = 0;
+  dsa_spa_workspace_bytes(p, &need);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u) != 0) return DSA_ERR_WORKSPACE;
+  if (p->kernel == DSA_KERNEL_TENSOR && !dsa_spa_uses_tensor_path(p)) return DSA_ERR_UNSUPPORTED;
+  cudaStream_t cs = (cudaStream_t)stream;
+  if (cudaMemsetAsync(workspace, 0, kWorkspaceHeader, cs) != cudaSuccess) return DSA_ERR_CUDA;
+  if (spa_rows(p) == 0) return DSA_OK;
+  return p->dtype == DSA_DTYPE_BF16 ? spa_launch_dense<__nv_bfloat16>(p, cs) : spa_launch_dense<__half>(p, cs);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -51,7 +51,8 @@ __device__ __forceinline__ int32_t sfa_slot_token(const SfaDev& p, const RowInfo
 
 // One query row, 16 heads starting at h0, by one block of 256 threads.
 // dynamic smem: (16 + 32) * (d + d_rope + pad) elements of T.
-template <typename T>
+// kDense: no indices, the row's slots are its visible keys (shared_prefix_attention).
+template <typename T, bool kDense = false>
 __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, int32_t h0) {
   extern __shared__ __align__(16) unsigned char sfa_smem[];
   const int32_t dq = p.d + p.d_rope;
@@ -108,8 +109,9 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
   if (tid < kSfaSimtHeads) { m_s[tid] = -INFINITY; l_s[tid] = 0.f; }
   __syncthreads();
 
-  const int32_t* idx_row = p.sparse_indices + (int64_t)row * p.sparse_count;
-  const int32_t slots = p.sparse_count * p.sparse_block_size;
+  const int32_t* idx_row = kDense ? nullptr : p.sparse_indices + (int64_t)row * p.sparse_count;
+  const int32_t slots = kDense ? ri.visible : p.sparse_count * p.sparse_block_size;
+  auto slot_token = [&](int32_t j) -> int32_t { return kDense ? j : sfa_slot_token(p, ri, idx_row, j); };
   const T* kn = (const T*)p.key;
   const T* kr = (const T*)p.key_rope;
 
@@ -121,7 +123,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
   __syncthreads();
   {
     int32_t part = 0;
-    for (int32_t j = tid; j < slots; j += kSfaSimtThreads) part += sfa_slot_token(p, ri, idx_row, j) >= 0;
+    for (int32_t j = tid; j < slots; j += kSfaSimtThreads) part += slot_token(j) >= 0;
     if (part) atomicAdd(&nvalid_s, part);
   }
   __syncthreads();
@@ -132,7 +134,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
     int any = 0;
     if (tid < kSfaSimtKeys) {
       int32_t j = j0 + tid;
-      int32_t tok = j < slots ? sfa_slot_token(p, ri, idx_row, j) : -1;
+      int32_t tok = j < slots ? slot_token(j) : -1;
       tok_s[tid] = tok;
       krow_s[tid] = tok >= 0 ? key_row(p.seq, ri, tok) : -1;
       any = tok >= 0;
@@ -270,15 +272,15 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
 }
 
 // grid = (rows, ceil(n1 / 16)); block = 256 threads.
-template <typename T>
+template <typename T, bool kDense = false>
 __global__ void __launch_bounds__(kSfaSimtThreads) sfa_fwd_mma_kernel(SfaDev p) {
-  sfa_fwd_mma_row<T>(p, (int32_t)blockIdx.x, (int32_t)blockIdx.y * kSfaSimtHeads);
+  sfa_fwd_mma_row<T, kDense>(p, (int32_t)blockIdx.x, (int32_t)blockIdx.y * kSfaSimtHeads);
 }
 
 // Recomputes the rows listed in redo_list[0 .. *redo_count) (rows whose scores outgrew the
 // tensor-core kernel's fixed reference maximum; normally none, and then every block leaves after
 // one load).  Any grid; blocks walk over (listed row, head chunk) pairs.
-template <typename T>
+template <typename T, bool kDense = false>
 __global__ void __launch_bounds__(kSfaSimtThreads) sfa_redo_kernel(SfaDev p, const int32_t* redo_list,
                                                                    const int32_t* redo_count) {
   grid_dep_wait();
@@ -286,7 +288,7 @@ __global__ void __launch_bounds__(kSfaSimtThreads) sfa_redo_kernel(SfaDev p, con
   const int64_t work = (int64_t)min(*redo_count, p.rows) * chunks;
   for (int64_t i = blockIdx.x; i < work; i += gridDim.x) {
     __syncthreads();   // the previous row's shared state is no longer read
-    sfa_fwd_mma_row<T>(p, redo_list[i / chunks], (int32_t)(i % chunks) * kSfaSimtHeads);
+    sfa_fwd_mma_row<T, kDense>(p, redo_list[i / chunks], (int32_t)(i % chunks) * kSfaSimtHeads);
   }
 }
 

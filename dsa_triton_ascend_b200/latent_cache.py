@@ -11,7 +11,7 @@ import torch
 
 from . import _cabi
 from ._host import current_stream, device_guard, dtype_code, ptr, require_cuda, same_device, seq_tensor
-from .rotary_embedding import check_inv_freq, check_positions, section_sizes
+from .rotary import check_inv_freq, check_positions, section_sizes
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
@@ -136,7 +136,7 @@ def latent_cache_append(
     if block_table.ndim != 2 or block_table.shape[0] != batch or tuple(seq_k.shape) != (batch,) or (
             seq_q is not None and tuple(seq_q.shape) != (batch,)):
         raise ValueError(f"block_table and lengths must have an entry for each of the {batch} sequences")
-    if latent.numel() == 0 or batch == 0:
+    if latent.numel() == 0 or batch == 0 or latent_cache.numel() == 0 or block_table.shape[1] == 0:
         return latent_cache, rope_cache, index_cache
     latent, key_rope = _token_rows(latent, 8, 16), _token_rows(key_rope, 2, 4)
     if index_key is not None:

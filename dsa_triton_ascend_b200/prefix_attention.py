@@ -1,0 +1,162 @@
+"""Attention over every visible key of the paged latent cache on B200, for a batch whose sequences share a prefix.
+
+No counterpart in the reference, whose attention takes selected keys (sparse_flash_attention_triton.py:1295-1455); layouts,
+lengths, statistics and checks are those of `sparse_flash_attention_triton`, with every visible key selected.
+"""
+import ctypes
+
+import torch
+
+from . import _cabi
+from ._host import (current_stream, device_guard, dtype_code, note_launch, packed, ptr, require_cuda, same_device,
+                    seq_tensor, workspace)
+
+_D, _D_ROPE = 512, 64
+_kernel = _cabi.KERNEL_AUTO
+
+
+def set_kernel(kind):
+    """"auto", "portable" (row by row) or "tensor" (tcgen05 path, error if not eligible)."""
+    global _kernel
+    _kernel = {"auto": _cabi.KERNEL_AUTO, "portable": _cabi.KERNEL_PORTABLE, "tensor": _cabi.KERNEL_TENSOR}[kind]
+
+
+def shared_prefix_attention(
+    query,
+    key,
+    scale_value: float = 1.0,
+    block_table=None,
+    actual_seq_lengths_query=None,
+    actual_seq_lengths_kv=None,
+    query_rope=None,
+    key_rope=None,
+    shared_prefix_length=0,
+    layout_query: str = "BSND",
+    sparse_mode: int = 3,
+    return_softmax_lse: bool = False,
+    block_size: int = 0,
+):
+    """MLA-absorb attention (one KV head, value = key) over the whole visible part of a paged cache.
+
+    Args:
+        query: [B,S1,N1,512] BSND or [T1,N1,512] TND, fp16/bf16, any number of heads
+        key:   [block_num,block_size,1,512], any block size
+        block_table: [B, max_blocks] int32, -1 = no block
+        actual_seq_lengths_query: [B] int32 / list / None (S1 each); cumulative, and required, for TND
+        actual_seq_lengths_kv: [B] int32 / list: cached keys of each sequence, the prefix counted
+        query_rope / key_rope: [..., 64], required
+        shared_prefix_length: how many first positions hold the same tokens in every sequence, an int or a
+            one-element int32 CUDA tensor (read when the call runs, so that a captured graph follows it).  They may be read
+            through any sequence's pages, so that they have to hold the same keys wherever a sequence has pages of its
+            own for them.  Sequences that do not see the whole prefix are computed from their own pages.  0: nothing is shared
+        sparse_mode: 0 full / 3 rightDownCausal
+        return_softmax_lse: also return the softmax statistics (zeros otherwise)
+        block_size: paged block length (defaults to key.shape[1])
+
+    Returns:
+        (attention_out, softmax_max, softmax_sum); statistics are fp32 [B,1,S1,N1] (BSND) or [1,T1,N1] (TND).  Rows that see
+        no key give zeros.  Serving only: paged caches are not differentiated.
+    """
+    if sparse_mode not in (0, 3):
+        raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")
+    if query_rope is None or key_rope is None:
+        raise ValueError("query_rope and key_rope are required (no empty rope)")
+    if layout_query not in ("BSND", "TND"):
+        raise ValueError(f"layout_query must be BSND or TND, got {layout_query}")
+    if block_table is None or actual_seq_lengths_kv is None:
+        raise ValueError("block_table and actual_seq_lengths_kv are required")
+    tnd = layout_query == "TND"
+    if query.ndim != (3 if tnd else 4):
+        raise ValueError(f"query must be {'[T1,N1,D]' if tnd else '[B,S1,N1,D]'}, got {tuple(query.shape)}")
+    if tnd and actual_seq_lengths_query is None:
+        raise ValueError("TND query requires cumulative actual_seq_lengths_query")
+    N1, D = query.shape[-2:]
+    if D != _D:
+        raise ValueError(f"D must be {_D}, got {D}")
+    if N1 < 1:
+        raise ValueError(f"N1 must be positive, got {N1}")
+    if tuple(query_rope.shape) != (*query.shape[:-1], _D_ROPE):
+        raise ValueError(f"query_rope must have shape {(*query.shape[:-1], _D_ROPE)}, got {tuple(query_rope.shape)}")
+    if key.ndim != 4 or key.shape[2] != 1 or key.shape[3] != D or key.shape[0] < 1 or key.shape[1] < 1:
+        raise ValueError(f"key must be [block_num,block_size,1,{D}] with a block at least, got {tuple(key.shape)}")
+    if tuple(key_rope.shape) != (*key.shape[:3], _D_ROPE):
+        raise ValueError(f"key_rope must have shape {(*key.shape[:3], _D_ROPE)}, got {tuple(key_rope.shape)}")
+    if (block_size or key.shape[1]) != key.shape[1]:
+        raise ValueError("block_size must equal the cache's block dimension")
+    if not (query.dtype == key.dtype == query_rope.dtype == key_rope.dtype):
+        raise ValueError("query, key, query_rope and key_rope must share a dtype")
+    code = dtype_code(query, (torch.bfloat16, torch.float16), "query")
+    prefix, prefix_t = shared_prefix_length, None
+    if isinstance(prefix, torch.Tensor):
+        if prefix.dtype != torch.int32 or prefix.numel() != 1:
+            raise ValueError("shared_prefix_length must be an int or a one-element int32 tensor")
+        prefix, prefix_t = 0, prefix
+    prefix = min(int(prefix), 2**31 - 1)
+    if prefix < 0:
+        raise ValueError(f"shared_prefix_length must not be negative, got {prefix}")
+    require_cuda(query, key, query_rope, key_rope, block_table, prefix_t)
+    same_device(query, key, query_rope, key_rope, block_table, prefix_t)
+    dev = query.device
+    seq_q, _ = seq_tensor(actual_seq_lengths_query, dev)
+    seq_k, _ = seq_tensor(actual_seq_lengths_kv, dev)
+    B = seq_q.shape[0] if tnd else query.shape[0]
+    block_table = block_table.to(dtype=torch.int32).contiguous()
+    if block_table.ndim != 2 or block_table.shape[0] != B or tuple(seq_k.shape) != (B,) or (
+            seq_q is not None and tuple(seq_q.shape) != (B,)):
+        raise ValueError(f"block_table and lengths must have an entry for each of the {B} sequences")
+    query, query_rope, key, key_rope = packed(query), packed(query_rope), packed(key), packed(key_rope)
+    s1 = query.shape[0] if tnd else query.shape[1]
+
+    out = torch.empty_like(query)
+    stat_shape = (1, s1, N1) if tnd else (B, 1, s1, N1)
+    sm_max = torch.empty(stat_shape, dtype=torch.float32, device=dev)
+    sm_sum = torch.empty(stat_shape, dtype=torch.float32, device=dev)
+    if out.numel() == 0:
+        return out, sm_max, sm_sum
+    if B == 0:      # tokens that belong to no sequence
+        return out.zero_(), sm_max.zero_(), sm_sum.zero_()
+
+    p = _cabi.DsaSpaParams()
+    p.struct_size = ctypes.sizeof(_cabi.DsaSpaParams)
+    p.kernel = _kernel
+    p.query, p.query_rope, p.key, p.key_rope = ptr(query), ptr(query_rope), ptr(key), ptr(key_rope)
+    p.seq_q, p.seq_k, p.block_table, p.prefix_device = ptr(seq_q), ptr(seq_k), ptr(block_table), ptr(prefix_t)
+    p.out, p.softmax_max, p.softmax_sum = ptr(out), ptr(sm_max), ptr(sm_sum)
+    p.layout_q, p.dtype = _cabi.LAYOUTS[layout_query], code
+    p.batch, p.s1, p.n1, p.d, p.d_rope = B, s1, N1, D, _D_ROPE
+    p.block_size, p.max_blocks = key.shape[1], block_table.shape[1]
+    p.prefix, p.sparse_mode = prefix, sparse_mode
+    p.return_lse = 1 if return_softmax_lse else 0
+    p.scale = float(scale_value)
+    p.key_rows = key.shape[0] * key.shape[1]
+    with device_guard(dev):
+        nbytes = ctypes.c_size_t(0)
+        _cabi.check(_cabi.lib.dsa_spa_workspace_bytes(ctypes.byref(p), ctypes.byref(nbytes)), "shared_prefix_attention")
+        ws = workspace(nbytes.value, dev)
+        _cabi.check(_cabi.lib.dsa_spa_forward(ctypes.byref(p), ws.data_ptr(), ws.numel(), current_stream(dev)),
+                    "shared_prefix_attention")
+        note_launch("shared_prefix_attention", ws, dev)
+    return out, sm_max, sm_sum
+
+
+class SharedPrefixAttention(torch.nn.Module):
+    """Attribute holder around shared_prefix_attention."""
+
+    def __init__(self, scale_value=1.0, layout_query="BSND", sparse_mode=3, return_softmax_lse=False, block_size=0):
+        super().__init__()
+        self.scale_value = scale_value
+        self.layout_query = layout_query
+        self.sparse_mode = sparse_mode
+        self.return_softmax_lse = return_softmax_lse
+        self.block_size = block_size
+
+    def forward(self, query, key, query_rope=None, key_rope=None, actual_seq_lengths_query=None,
+                actual_seq_lengths_kv=None, block_table=None, shared_prefix_length=0):
+        return shared_prefix_attention(
+            query, key, scale_value=self.scale_value, block_table=block_table,
+            actual_seq_lengths_query=actual_seq_lengths_query, actual_seq_lengths_kv=actual_seq_lengths_kv,
+            query_rope=query_rope, key_rope=key_rope, shared_prefix_length=shared_prefix_length,
+            layout_query=self.layout_query, sparse_mode=self.sparse_mode, return_softmax_lse=self.return_softmax_lse,
+            block_size=self.block_size)
+
+    construct = forward

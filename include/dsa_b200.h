@@ -382,6 +382,48 @@ typedef struct DsaAppendParams {
 } DsaAppendParams;
 int dsa_latent_append(const DsaAppendParams* p, void* stream);
 
+/*
+ * Attention of query tokens over every visible key of a paged latent cache, MLA-absorb (value = key[..., :d]), one
+ * KV head, for a batch whose sequences begin with the same tokens (no counterpart in the reference).
+ *
+ *   out[t, h] = sum_p softmax_p(scale * (query[t, h] . key[p] + query_rope[t, h] . key_rope[p])) key[p]
+ * over the positions p < visible(t) of the token's sequence: seq_k (mode 0) or seq_k - seq_q + position + 1 (mode 3).
+ * seq_k counts the prefix.  The first `prefix` positions of every sequence hold the same keys (the caller's promise):
+ * they may be read through any sequence's row of the block table.  prefix_device, if not NULL, is read in place of
+ * `prefix` when the call runs.  A length past a sequence's own is no error: a sequence that does not see the whole prefix is
+ * computed from its own pages.  prefix = 0: plain attention over the paged cache.  Blocks that are absent (-1) or beyond the
+ * cache inside a valid length read as zero keys that take part.  Rows without a visible key, padding rows and rows
+ * behind the last sequence give zeros in all three outputs.
+ */
+typedef struct DsaSpaParams {
+  uint32_t struct_size; /* sizeof(DsaSpaParams) */
+  int32_t kernel;         /* DSA_KERNEL_*         */
+  const void* query;      /* [rows, n1, d]        */
+  const void* query_rope; /* [rows, n1, d_rope]   */
+  const void* key;        /* [blocks, block_size, 1, d]      */
+  const void* key_rope;   /* [blocks, block_size, 1, d_rope] */
+  const int32_t* seq_q;   /* BSND: [batch] lengths or NULL; TND: cumulative ends */
+  const int32_t* seq_k;   /* [batch] lengths      */
+  const int32_t* block_table;   /* [batch, max_blocks], -1 = no block */
+  const int32_t* prefix_device; /* [1] or NULL    */
+  void* out;              /* [rows, n1, d], dtype */
+  float* softmax_max;     /* [rows, n1]; both or neither may be NULL */
+  float* softmax_sum;
+  int32_t layout_q, dtype;
+  int32_t batch, s1;      /* BSND: S1; TND: total query tokens T1 */
+  int32_t n1, d, d_rope;  /* d = 512, d_rope = 64 */
+  int32_t block_size, max_blocks;
+  int32_t prefix;         /* >= 0 */
+  int32_t sparse_mode;    /* 0 full, 3 rightDownCausal */
+  int32_t return_lse;     /* 0: zeros are stored as statistics */
+  float scale;
+  int64_t key_rows;       /* blocks * block_size */
+} DsaSpaParams;
+int dsa_spa_workspace_bytes(const DsaSpaParams* p, size_t* out_bytes);
+int dsa_spa_forward(const DsaSpaParams* p, void* workspace, size_t workspace_bytes, void* stream);
+/* 1 when dsa_spa_forward would take the tcgen05 path for these parameters, else 0. */
+int dsa_spa_uses_tensor_path(const DsaSpaParams* p);
+
 /* Static description of a status code. */
 const char* dsa_status_string(int status);
 /* Synchronises `stream` and returns the device status word stored at the start of a

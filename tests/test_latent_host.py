@@ -26,7 +26,7 @@ def _layout(struct):
     assert out[1:] == [getattr(cls, n).offset for n in fields]
 
 
-@pytest.mark.parametrize("struct", ["DsaRopeParams", "DsaAppendParams"])
+@pytest.mark.parametrize("struct", ["DsaRopeParams", "DsaAppendParams", "DsaSpaParams"])
 def test_struct_layouts(struct):
     _layout(struct)
 
@@ -132,3 +132,62 @@ def test_c_interface_refuses_bad_arguments_without_a_gpu():
     assert call(_cabi.lib.dsa_latent_append, a) == -3
     a.index_offset, a.max_blocks, a.block_size = 64, 1 << 20, 1 << 12
     assert call(_cabi.lib.dsa_latent_append, a) == -8
+
+
+def _attend(**kw):
+    from dsa_triton_ascend_b200 import shared_prefix_attention
+    z = lambda *s: torch.zeros(*s, dtype=BF)
+    a = dict(query=z(2, 1, 4, 512), key=z(4, 16, 1, 512), query_rope=z(2, 1, 4, 64), key_rope=z(4, 16, 1, 64),
+             block_table=torch.zeros(2, 2, dtype=torch.int32), actual_seq_lengths_kv=[3, 3])
+    a.update(kw)
+    return shared_prefix_attention(**a)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(sparse_mode=1), dict(query_rope=None), dict(key_rope=None), dict(layout_query="PA_BSND"), dict(layout_query="TND"),
+    dict(block_table=None), dict(actual_seq_lengths_kv=None), dict(query=torch.zeros(2, 1, 4, 256, dtype=BF)),
+    dict(query=torch.zeros(2, 1, 0, 512, dtype=BF)), dict(query_rope=torch.zeros(2, 1, 4, 32, dtype=BF)),
+    dict(query_rope=torch.zeros(2, 1, 3, 64, dtype=BF)), dict(key=torch.zeros(4, 16, 2, 512, dtype=BF)),
+    dict(key=torch.zeros(0, 16, 1, 512, dtype=BF)), dict(key=torch.zeros(4, 16, 512, dtype=BF)),
+    dict(key_rope=torch.zeros(4, 8, 1, 64, dtype=BF)), dict(key_rope=torch.zeros(4, 16, 1, 64, dtype=torch.float16)),
+    dict(block_size=32), dict(shared_prefix_length=-1), dict(shared_prefix_length=torch.zeros(1)),
+    dict(shared_prefix_length=torch.zeros(2, dtype=torch.int32)),
+])
+def test_attention_refusals(kw):
+    with pytest.raises(ValueError):
+        _attend(**kw)
+
+
+def test_attention_refuses_cpu_tensors():
+    with pytest.raises(RuntimeError):
+        _attend()
+
+
+def test_attention_c_interface_refuses_bad_arguments_without_a_gpu():
+    from dsa_triton_ascend_b200 import _cabi
+    n, p = ctypes.c_size_t(0), _cabi.DsaSpaParams()
+    size = lambda: _cabi.lib.dsa_spa_workspace_bytes(ctypes.byref(p), ctypes.byref(n))
+    assert size() == -2
+    p.struct_size = ctypes.sizeof(p)
+    assert size() == -1
+    p.query = p.query_rope = p.key = p.key_rope = p.seq_k = p.block_table = p.out = 256
+    p.batch, p.s1, p.n1, p.d, p.d_rope, p.block_size, p.max_blocks, p.key_rows = 2, 1, 4, 512, 64, 16, 2, 64
+    assert size() == 0 and n.value >= 256
+    for name, bad in (("d", 256), ("d_rope", 0), ("dtype", 2), ("batch", 0), ("n1", 0), ("block_size", 0), ("prefix", -1),
+                      ("key_rows", 0), ("sparse_mode", 1), ("kernel", 3), ("key", 264), ("key_rope", 258), ("layout_q", 2)):
+        old = getattr(p, name)
+        setattr(p, name, bad)
+        assert size() == -3, name
+        setattr(p, name, old)
+    for name, bad in (("max_blocks", 1 << 28), ("s1", 1 << 30)):
+        old = getattr(p, name)
+        setattr(p, name, bad)
+        assert size() == -8, name
+        setattr(p, name, old)
+    p.layout_q = 1
+    assert size() == -1          # TND without cumulative lengths
+    p.layout_q, p.return_lse = 0, 1
+    assert size() == -1          # statistics asked for, nowhere to put them
+    p.return_lse = 0
+    assert _cabi.lib.dsa_spa_forward(ctypes.byref(p), None, 0, None) == -4
+    assert _cabi.lib.dsa_spa_forward(ctypes.byref(p), 128, 1 << 30, None) == -4
