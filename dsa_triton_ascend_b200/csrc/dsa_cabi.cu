@@ -14,6 +14,7 @@
 #include "rope.cuh"
 #include "sfa_fwd_mma.cuh"
 #include "sfa_fwd_sm100.cuh"
+#include "spa_sm100.cuh"
 #include "sfa_bwd_simt.cuh"
 #include "sfa_bwd_mma.cuh"
 #include "sfa_bwd_sm100.cuh"
@@ -1015,13 +1016,16 @@ int dsa_li_forward_static(const DsaLiParams* p, void* stream) {
 // ---------------------------------------------------------------------------------------------
 // Attention over the paged latent cache behind a shared prefix
 // ---------------------------------------------------------------------------------------------
-int dsa_spa_uses_tensor_path(const DsaSpaParams* p) { return 0; }
+int dsa_spa_uses_tensor_path(const DsaSpaParams* p) {
+  if (spa_validate(p) != DSA_OK) return 0;
+  return p->kernel != DSA_KERNEL_PORTABLE && spa_sm100_eligible(p, spa_rows(p)) ? 1 : 0;
+}
 
 int dsa_spa_workspace_bytes(const DsaSpaParams* p, size_t* out_bytes) {
   const int rc = spa_validate(p);
   if (rc != DSA_OK) return rc;
   if (!out_bytes) return DSA_ERR_NULL;
-  *out_bytes = kWorkspaceHeader;
+  *out_bytes = kWorkspaceHeader + (dsa_spa_uses_tensor_path(p) ? spa_ws_layout(p, spa_rows(p)).total : 0);
   return DSA_OK;
 }
 
@@ -1033,6 +1037,8 @@ int dsa_spa_forward(const DsaSpaParams* p, void* workspace, size_t workspace_byt
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u) != 0) return DSA_ERR_WORKSPACE;
   if (p->kernel == DSA_KERNEL_TENSOR && !dsa_spa_uses_tensor_path(p)) return DSA_ERR_UNSUPPORTED;
   cudaStream_t cs = (cudaStream_t)stream;
+  if (dsa_spa_uses_tensor_path(p))   // (the plan kernel clears the header)
+    return spa_sm100_launch(p, spa_dense_dev(p), (int32_t*)workspace, (char*)workspace + kWorkspaceHeader, cs);
   if (cudaMemsetAsync(workspace, 0, kWorkspaceHeader, cs) != cudaSuccess) return DSA_ERR_CUDA;
   if (spa_rows(p) == 0) return DSA_OK;
   return p->dtype == DSA_DTYPE_BF16 ? spa_launch_dense<__nv_bfloat16>(p, cs) : spa_launch_dense<__half>(p, cs);

@@ -1,0 +1,985 @@
+// Attention over the paged latent cache behind a shared prefix, on tcgen05: MLA-absorb, D = 512 (+64 rope), one KV head, any
+// number of heads, any page size.
+//
+// Rows.  A row is a (token, head) pair; rows are flat in memory (token * n1 + head), so that 128 consecutive ones are one
+// M = 128 tile whatever the number of heads.  A job is a row tile against a range of key positions:
+//   - a sequence of few rows (up to 64) that sees the whole prefix is PACKED: its rows meet the prefix together with those
+//     of its neighbours, in tiles cut from the flat rows of the whole batch (prefix jobs), and its own keys in a job of its own;
+//   - every other sequence is cut into row tiles of its own, each over all the tile's visible keys.  Its tiles are full (or
+//     nearly), so that packing would save nothing; that the prefix is the same pages for everybody then shows as L2 hits.
+// A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into equal
+// shares, one per CTA pair, in the order of the jobs: every pair works for the same time whatever the lengths are.  A job that
+// lies in one pair's share and has no other part writes its result; the others leave normalised fp32 partials
+// (maximum, sum, O) that spa_join_kernel adds up in a fixed order.  One block of rows has
+//   out = sum_i w_i O_i / sum_i w_i,   w_i = l_i exp(m_i - max m).
+//
+// Products.  A CTA pair works on a tile with tcgen05.mma.cta_group::2, M = 128 = 2 x 64 rows: S = Q K^T (N = 128 keys, B
+// split along the keys: CTA c loads keys 64 c .. 64 c + 63 with all 576 features) and O += P V (two N = 256 products per 16
+// keys, B split along the value columns: CTA c loads all 128 keys x columns {c 128 .., 256 + c 128 ..}).  Such a product
+// with A (64 rows a CTA) in shared memory takes 16 + N / 4 cycles per 16 of K: 36 x 48 + 16 x 80 = 3008 cycles for a tile
+// of 128 keys, against 2176 at the full rate and 3584 as two tiles of 64.
+// Tensor memory: lanes 0..63 hold a CTA's rows with the first half of N, lanes 64..127 the same rows with the second:
+// S buffers 2 x 64 columns, O 256.
+//
+// Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, 16 of them per box where the page size is a
+// multiple of 16, else (and at the ends of a range, where some of 16 are not wanted) with gather4, four rows each; rows
+// that are not wanted and absent pages are read at a row past the tensor, which gives zeros without touching
+// memory: what lies behind a sequence's end never enters a product.  Bytes are counted on the even CTA's barriers, where
+// the products are issued.  Rings: K 9 blocks of 64 keys x 64 features, V 8 blocks of 16 keys x 256 columns, each of one
+// tile, refilled block by block.
+//
+// Softmax.  Eight warps take every tile together: the four threads of a row (two halves of N x two groups of 32 keys)
+// exchange their maxima through shared memory.  P is relative to a running reference that follows the maximum only when it is
+// exceeded by more than 2^8: then O is rescaled in tensor memory (P <= 2^8 fits both types, the sums are fp32).
+// Rows of one tile may see different numbers of keys (causal tokens of one sequence).  A hidden key has P = 0, and
+// 0 x infinity would be NaN: a hidden key whose score is not finite (every non-finite latent makes it so, for every row)
+// marks the token, and sfa_redo_kernel computes it again from its visible keys alone.  Normally no token.
+//
+// Warps (416 threads): 0 K loads, 1 V loads, 2 Q loads and tensor memory, 3 QK issuer, 4..11 softmax, 12 PV issuer.
+// All waits are bounded; one that gives up sets the status word.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "ptx_sm100.cuh"
+#include "sfa_fwd_mma.cuh"
+#include "sfa_fwd_sm100.cuh"
+
+namespace dsa {
+
+constexpr int kSpaRows = 128;        // rows per tile (64 per CTA)
+constexpr int kSpaKeys = 128;        // keys per tile
+constexpr int kSpaThreads = 416;
+constexpr int kSpaSoftWarp0 = 4, kSpaPvWarp = 12;
+constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
+constexpr int kSpaPackKeys = 256;    // a shorter prefix is not worth the partials
+constexpr int kSpaPlanThreads = 1024;
+
+constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
+constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
+constexpr uint32_t kSpaBlk = 8192;                          // a K block (64 keys x 64 features) or V block (16 keys x 256 columns)
+constexpr uint32_t kSpaPBlk = 64 * 128;                     // 64 rows x 64 keys
+constexpr uint32_t kSpaOffQ = 0;
+constexpr uint32_t kSpaOffK = kSpaOffQ + kSpaQBytes;
+constexpr uint32_t kSpaOffV = kSpaOffK + 9 * kSpaBlk;
+constexpr uint32_t kSpaOffP = kSpaOffV + 8 * kSpaBlk;
+constexpr uint32_t kSpaOffX = kSpaOffP + 2 * kSpaPBlk;      // float [2][4][64]
+constexpr uint32_t kSpaOffBar = kSpaOffX + 2048;
+constexpr uint32_t kSpaSmemBytes = kSpaOffBar + 512;
+static_assert(kSpaSmemBytes <= 232448, "shared memory");
+constexpr uint32_t kSpaTmO = 0, kSpaTmS = 256;
+constexpr float kSpaGuard = 8.f;     // log2 units that a score may exceed the reference by
+
+// One row tile against positions lo .. hi - 1, in tiles of 128 keys that start at key0.
+struct SpaJob {
+  int32_t row0, nrows;      // flat rows
+  int32_t table_row;        // whose row of the block table the positions are looked up in
+  int32_t key0, lo, hi;
+  int32_t tile0, tiles;     // first tile in the order of all jobs' tiles, and their number
+  int32_t vis0;             // positions that the first row's token sees (mode 3: one more per token)
+  int32_t head0;            // head of the first row
+  int32_t packed;           // 1: rows of packed sequences against the prefix; the rows of other sequences are skipped
+  int32_t slot;             // partial that the whole job leaves; -1: it writes its result
+};
+static_assert(sizeof(SpaJob) == 48, "three 16-byte loads");
+
+struct SpaPlan {
+  int32_t jobs, tiles, share;   // share: tiles per CTA pair
+  int32_t prefix, ref;          // positions shared, and the sequence whose pages they are read from
+};
+
+struct SpaDev {
+  SeqDesc seq;              // seq_k: keys with the prefix; paged
+  const int32_t* prefix_device;
+  int32_t prefix;
+  int32_t rows, n1;         // tokens, heads
+  int32_t prefix_tiles, own_tiles, own_tiles_per_seq;   // places in the list of row tiles (own_tiles_per_seq: BSND)
+  int32_t pack_rows;        // kSpaPackRows, or 0 when nothing may be packed
+  int32_t clusters;
+  // workspace
+  SpaPlan* plan;
+  SpaJob* job;              // [prefix_tiles + own_tiles]
+  int32_t* job_of;          // [prefix_tiles + own_tiles] job of a row tile, -1: none
+  int32_t* first_job;       // [clusters] job of a pair's first tile
+  int32_t* redo;            // [rows]
+  int32_t* redo_list;       // [rows]
+  int32_t* redo_count;
+  int32_t* status;
+  float* part_o;            // [slots, 128, 512]
+  float* part_m;            // [slots, 128] maximum of the scaled scores, log2 units
+  float* part_l;            // [slots, 128] sum relative to it; 0: the row takes no part
+  // outputs
+  void* out;
+  float* softmax_max;
+  float* softmax_sum;
+  int32_t return_lse;
+};
+
+// What the plan and the kernels that follow it agree on about a sequence.
+struct SpaSeq {
+  int32_t start, act_q, act_k;   // first token, query tokens (within the tensor), keys (within the table)
+  int32_t vis0;                  // positions that its first token sees (may be negative)
+  bool packed;
+};
+__device__ __forceinline__ SpaSeq spa_seq(const SpaDev& p, int32_t b, int32_t prefix) {
+  SpaSeq s;
+  int32_t act_q;
+  if (p.seq.layout_q == DSA_LAYOUT_TND) {
+    s.start = b > 0 ? p.seq.seq_q[b - 1] : 0;
+    act_q = p.seq.seq_q[b] - s.start;
+    s.start = min(max(s.start, 0), p.rows);
+    s.act_q = max(0, min(act_q, p.rows - s.start));
+  } else {
+    s.start = b * p.seq.s1;
+    act_q = p.seq.seq_q ? p.seq.seq_q[b] : p.seq.s1;
+    s.act_q = max(0, min(act_q, p.seq.s1));
+  }
+  const int32_t act_k = p.seq.seq_k[b];
+  s.act_k = max(0, min(act_k, p.seq.s2));
+  // (the mask counts with the lengths as they were given)
+  s.vis0 = p.seq.sparse_mode == 3 ? (int32_t)max((int64_t)-0x40000000, (int64_t)act_k - act_q + 1) : s.act_k;
+  s.packed = prefix >= kSpaPackKeys && s.act_q > 0 && (int64_t)s.act_q * p.n1 <= p.pack_rows && s.act_k >= prefix &&
+             s.vis0 >= prefix;
+  return s;
+}
+// First place of a sequence's row tiles in the list (behind the prefix tiles).
+__device__ __forceinline__ int32_t spa_own_place(const SpaDev& p, int32_t b, int32_t start) {
+  if (p.seq.layout_q != DSA_LAYOUT_TND) return b * p.own_tiles_per_seq;
+  return (int32_t)((int64_t)start * p.n1 / kSpaRows) + b;
+}
+
+// ---- plan: one block ------------------------------------------------------------------------------
+__global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev p) {
+  __shared__ unsigned long long best_s[32];
+  __shared__ int32_t sum_s[3][33];
+  __shared__ int32_t total_s[3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_dep_launch();
+  grid_dep_wait();
+  if (tid < 64) p.status[tid] = 0;
+  if (p.redo != nullptr) {
+    if (tid == 0) *p.redo_count = 0;
+    for (int32_t i = tid; i < p.rows; i += kSpaPlanThreads) p.redo[i] = 0;
+  }
+  // the longest sequence (the first of them) lends its pages for the prefix
+  unsigned long long best = 0;
+  for (int32_t b = tid; b < p.seq.batch; b += kSpaPlanThreads) {
+    const int32_t k = max(0, min(p.seq.seq_k[b], p.seq.s2));
+    best = max(best, ((unsigned long long)(uint32_t)k << 32) | (uint32_t)(0x7FFFFFFF - b));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) best_s[warp] = best;
+  __syncthreads();
+  best = best_s[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  const int32_t longest = (int32_t)(best >> 32), ref = 0x7FFFFFFF - (int32_t)(uint32_t)best;
+  int32_t prefix = p.prefix_device ? *p.prefix_device : p.prefix;
+  prefix = max(0, min(prefix, longest));
+
+  const int32_t places = p.prefix_tiles + p.own_tiles, rows = p.rows * p.n1;
+  int32_t jobs = 0, tiles = 0, packed = 0;   // listed so far
+  for (int32_t f0 = 0; f0 < places; f0 += kSpaPlanThreads) {
+    const int32_t f = f0 + tid;
+    SpaJob j;
+    j.tiles = 0;
+    j.slot = -1;
+    if (f < p.prefix_tiles) {
+      j.row0 = f * kSpaRows;
+      j.nrows = min(kSpaRows, rows - j.row0);
+      // does any of its rows belong to a packed sequence?
+      const int32_t t0 = j.row0 / p.n1, t1 = (j.row0 + j.nrows - 1) / p.n1;
+      int32_t b = 0;
+      bool any = false;
+      if (prefix >= kSpaPackKeys) {
+        const RowInfo ri = row_info(p.seq, t0);
+        for (b = ri.b; b < p.seq.batch && !any; ++b) {
+          const SpaSeq s = spa_seq(p, b, prefix);
+          if (s.start > t1) break;
+          any = s.packed && s.start + s.act_q > t0;
+        }
+      }
+      j.table_row = ref;
+      j.key0 = 0; j.lo = 0; j.hi = prefix;
+      j.vis0 = prefix;
+      j.head0 = j.row0 % p.n1;
+      j.packed = 1;
+      if (any) j.tiles = (prefix + kSpaKeys - 1) / kSpaKeys;
+      j.slot = 0;
+    } else if (f < places) {
+      const int32_t g = f - p.prefix_tiles;
+      int32_t b;
+      if (p.seq.layout_q != DSA_LAYOUT_TND) b = g / p.own_tiles_per_seq;
+      else {
+        int32_t lo = 0, hi = p.seq.batch - 1;      // the last sequence whose first place is g or before
+        while (lo < hi) {
+          const int32_t mid = (lo + hi + 1) >> 1;
+          if (spa_own_place(p, mid, min(max(p.seq.seq_q[mid - 1], 0), p.rows)) <= g) lo = mid; else hi = mid - 1;
+        }
+        b = lo;
+      }
+      const SpaSeq s = spa_seq(p, b, prefix);
+      const int32_t i = g - spa_own_place(p, b, s.start), n = s.act_q * p.n1;
+      j.row0 = s.start * p.n1 + i * kSpaRows;
+      j.nrows = min(kSpaRows, n - i * kSpaRows);
+      if (i >= 0 && j.nrows > 0) {
+        const int32_t first = i * kSpaRows / p.n1, last = (i * kSpaRows + j.nrows - 1) / p.n1;   // its tokens
+        j.table_row = b;
+        j.lo = s.packed ? prefix : 0;
+        j.hi = p.seq.sparse_mode == 3 ? min(s.vis0 + last, s.act_k) : s.act_k;
+        j.key0 = j.lo & ~(kSpaKeys - 1);
+        j.vis0 = p.seq.sparse_mode == 3 ? s.vis0 + first : s.act_k;
+        j.head0 = i * kSpaRows % p.n1;
+        j.packed = 0;
+        if (j.hi > j.lo) j.tiles = (j.hi - j.key0 + kSpaKeys - 1) / kSpaKeys;
+        j.slot = s.packed ? 0 : -1;
+      }
+    }
+    // running sums over the block: jobs, tiles, jobs that leave a partial
+    const int32_t v[3] = {j.tiles > 0, j.tiles, j.tiles > 0 && j.slot == 0};
+    int32_t x[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      x[k] = v[k];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t y = __shfl_up_sync(0xffffffffu, x[k], o);
+        if (lane >= o) x[k] += y;
+      }
+      if (lane == 31) sum_s[k][warp] = x[k];
+    }
+    __syncthreads();
+    if (warp < 3) {
+      const int32_t mine = sum_s[warp][lane];
+      int32_t z = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t y = __shfl_up_sync(0xffffffffu, z, o);
+        if (lane >= o) z += y;
+      }
+      sum_s[warp][lane] = z - mine;
+      if (lane == 31) total_s[warp] = z;
+    }
+    __syncthreads();
+    if (f < places) {
+      const int32_t at = jobs + sum_s[0][warp] + x[0] - v[0];
+      p.job_of[f] = v[0] ? at : -1;
+      if (v[0]) {
+        j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1];
+        if (v[2]) j.slot = 2 * p.clusters + packed + sum_s[2][warp] + x[2] - v[2];
+        p.job[at] = j;
+      }
+    }
+    jobs += total_s[0]; tiles += total_s[1]; packed += total_s[2];
+    __syncthreads();
+  }
+  const int32_t share = max(1, (tiles + p.clusters - 1) / p.clusters);
+  if (tid == 0) {
+    SpaPlan w;
+    w.jobs = jobs; w.tiles = tiles; w.share = share; w.prefix = prefix; w.ref = ref;
+    *p.plan = w;
+  }
+  for (int32_t i = tid; i < jobs; i += kSpaPlanThreads) {
+    const int32_t t0 = p.job[i].tile0, t1 = t0 + p.job[i].tiles;
+    for (int32_t c = (t0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) p.first_job[c] = i;
+  }
+}
+
+// Where the tiles a .. b - 1 of a job leave their result: -1 in the output, else a partial.  A pair's share has at most one
+// job that began before it and one more that goes on after it.
+__device__ __forceinline__ int32_t spa_slot(const SpaJob& j, int32_t a, int32_t b, int32_t cluster) {
+  if (a == 0 && b == j.tiles) return j.slot;
+  return 2 * cluster + (a > 0 ? 0 : 1);
+}
+
+__device__ __forceinline__ SpaJob spa_load_job(const SpaJob* p) {
+  SpaJob j;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) reinterpret_cast<int4*>(&j)[i] = reinterpret_cast<const int4*>(p)[i];
+  return j;
+}
+
+// Walks over the tiles of a pair's share.
+struct SpaWalk {
+  const SpaJob* jobs;
+  int32_t at, end, index;    // tile in the order of all tiles, end of the share, job
+  SpaJob j;
+  __device__ __forceinline__ void start(const SpaDev& p, int32_t cluster) {
+    const SpaPlan w = *p.plan;
+    jobs = p.job;
+    at = min((int64_t)cluster * w.share, (int64_t)w.tiles);
+    end = min(at + w.share, w.tiles);
+    index = 0;
+    if (at < end) { index = p.first_job[cluster]; j = spa_load_job(jobs + index); }
+  }
+  __device__ __forceinline__ bool more() const { return at < end; }
+  __device__ __forceinline__ int32_t tile() const { return at - j.tile0; }                       // of the job
+  __device__ __forceinline__ int32_t stop() const { return min(j.tiles, end - j.tile0); }        // tile of the job to stop at
+  __device__ __forceinline__ void next_tile() {
+    if (++at < end && at >= j.tile0 + j.tiles) j = spa_load_job(jobs + ++index);
+  }
+  __device__ __forceinline__ void next_job() {
+    at = j.tile0 + stop();
+    if (at < end) j = spa_load_job(jobs + ++index);
+  }
+};
+
+struct SpaArgs {
+  SpaDev p;
+  uint32_t idesc_qk, idesc_pv;
+  float scale_log2;
+  int32_t is_bf16, key_rows;
+};
+
+// The four rows of the cache at positions pos .. pos + 3 of a job (key_rows, past the tensor: zeros).
+struct SpaQuad { int32_t r[4]; bool box; };
+__device__ __forceinline__ SpaQuad spa_quad(const SpaArgs& a, const SpaJob& j, int32_t pos) {
+  const int32_t bs = a.p.seq.block_size;
+  const int32_t* table = a.p.seq.block_table + (int64_t)j.table_row * a.p.seq.max_blocks;
+  const int32_t blocks = a.key_rows / bs;
+  SpaQuad q;
+  const int32_t first = pos & ~15;
+  const bool whole = (bs & 15) == 0;
+  q.box = whole && first >= j.lo && first + 16 <= j.hi;
+  int32_t page = -1, blk = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int32_t x = pos + i;
+    q.r[i] = a.key_rows;
+    if (x >= j.lo && x < j.hi) {
+      const int32_t g = x / bs;
+      if (g != page) { page = g; blk = table[g]; }
+      if (blk >= 0 && blk < blocks) q.r[i] = blk * bs + (x - g * bs);
+    }
+  }
+  return q;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSpaThreads, 1)
+spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_qr,
+                     const __grid_constant__ CUtensorMap tmap_k16, const __grid_constant__ CUtensorMap tmap_r16,
+                     const __grid_constant__ CUtensorMap tmap_k1, const __grid_constant__ CUtensorMap tmap_r1,
+                     const SpaArgs a) {
+  extern __shared__ __align__(1024) unsigned char spa_sm[];
+  unsigned char* q_s = spa_sm + kSpaOffQ;
+  unsigned char* k_s = spa_sm + kSpaOffK;
+  unsigned char* v_s = spa_sm + kSpaOffV;
+  unsigned char* p_s = spa_sm + kSpaOffP;
+  float* xm = reinterpret_cast<float*>(spa_sm + kSpaOffX);      // [2 turns][4 threads of a row][64 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(spa_sm + kSpaOffBar);
+  uint64_t* k_full = bars;         // [9] even CTA: both CTAs' blocks have landed (bytes)
+  uint64_t* k_empty = bars + 9;    // [9] the products that read the block are done (commit, both CTAs)
+  uint64_t* v_full = bars + 18;    // [8]
+  uint64_t* v_empty = bars + 26;   // [8]
+  uint64_t* q_full = bars + 34;    // even CTA: both CTAs' rows have landed
+  uint64_t* q_empty = bars + 35;   // the job's last score product is done (commit, both CTAs)
+  uint64_t* s_full = bars + 36;    // [2] scores of a tile are done (commit, both CTAs)
+  uint64_t* s_empty = bars + 38;   // [2] even CTA: the softmax warps of both CTAs hold them in registers
+  uint64_t* p_full = bars + 40;    // even CTA: P stored in both CTAs, O rescaled where it had to be
+  uint64_t* p_empty = bars + 41;   // the tile's value products are done (commit, both CTAs)
+  uint64_t* o_free = bars + 42;    // even CTA: the softmax warps of both CTAs have read O
+  uint64_t* x_bar = bars + 43;     // [2] xm written: the four warps that hold the same 32 rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 45);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 46);
+  static_assert(47 * 8 <= 512, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const int32_t cluster = blockIdx.x >> 1;
+
+  const bool misaligned = (ptx::smem_u32(spa_sm) & 1023u) != 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 9; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 8; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
+    ptx::mbar_init(q_full, 1);
+    ptx::mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&s_empty[i], 16); ptx::mbar_init(&x_bar[i], 4);
+    }
+    ptx::mbar_init(p_full, 16);
+    ptx::mbar_init(p_empty, 1);
+    ptx::mbar_init(o_free, 16);
+    *abort_flag = misaligned ? 1 : 0;
+    ptx::mbar_fence_init();
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc_pair(tmem_slot, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  ptx::cluster_arrive();     // the peer's barriers must exist before anything is sent to it
+  ptx::cluster_wait();
+  grid_dep_launch();
+  grid_dep_wait();           // (nothing before this touches global memory)
+  const uint32_t tmem = *tmem_slot;
+
+  if (*abort_flag) {
+    // nothing started
+  } else if (warp == 0) {
+    // ------------------------------------------------------------------ K loads
+    // Lane 4 g + i of the first 16 holds positions 16 g + 4 i .. + 3 of this CTA's 64; a group of 16 is one box per block.
+    const uint32_t dst0 = ptx::smem_u32(k_s) + (lane >> 2) * 2048;
+    SpaWalk w;
+    w.start(a.p, cluster);
+    SpaQuad cur = {};
+    auto quad = [&](const SpaWalk& x) {
+      if (x.more() && lane < 16) cur = spa_quad(a, x.j, x.j.key0 + x.tile() * kSpaKeys + (int32_t)rank * 64 + lane * 4);
+    };
+    quad(w);
+    bool ok = true;
+    for (uint32_t n = 0; w.more() && ok; ++n) {
+      const SpaQuad q = cur;
+      w.next_tile();
+      quad(w);              // (the look-ups of the next tile are in flight while this one is waited for)
+#pragma unroll 1
+      for (int f = 0; f < 9 && ok; ++f) {
+        ok = ptx::mbar_spin_warp(&k_empty[f], (n & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[f], 2 * kSpaBlk);
+        const uint32_t bar = ptx::map_to_rank(&k_full[f], 0);
+        const uint32_t dst = dst0 + f * kSpaBlk;
+        const int32_t x = f < 8 ? f * 64 : 0;
+        if (lane < 16) {
+          if (!q.box) ptx::tma_gather4_2d_pair(dst + (lane & 3) * 512, f < 8 ? &tmap_k1 : &tmap_r1, bar, x, q.r[0], q.r[1], q.r[2], q.r[3]);
+          else if ((lane & 3) == 0) ptx::tma_load_2d_pair(dst, f < 8 ? &tmap_k16 : &tmap_r16, bar, x, q.r[0]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ V loads
+    // Lane 4 g + i holds positions 16 g + 4 i .. + 3 of the tile's 128; group g is block g of the ring, and where it is
+    // whole pages' rows, lane i of it loads its column block i.
+    SpaWalk w;
+    w.start(a.p, cluster);
+    SpaQuad cur = {};
+    auto quad = [&](const SpaWalk& x) {
+      if (x.more()) cur = spa_quad(a, x.j, x.j.key0 + x.tile() * kSpaKeys + lane * 4);
+    };
+    quad(w);
+    bool ok = true;
+    for (uint32_t n = 0; w.more() && ok; ++n) {
+      const SpaQuad q = cur;
+      w.next_tile();
+      quad(w);
+      const int32_t row0 = __shfl_sync(0xffffffffu, q.r[0], lane & ~3);
+#pragma unroll 1
+      for (int g = 0; g < 8 && ok; ++g) {
+        ok = ptx::mbar_spin_warp(&v_empty[g], (n & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[g], 2 * kSpaBlk);
+        const uint32_t bar = ptx::map_to_rank(&v_full[g], 0);
+        if ((lane >> 2) == g) {
+          const uint32_t dst = ptx::smem_u32(v_s) + g * kSpaBlk;
+          const int i = lane & 3;
+          if (q.box) {
+            ptx::tma_load_2d_pair(dst + i * 2048, &tmap_k16, bar, (i >> 1) * 256 + (int32_t)rank * 128 + (i & 1) * 64, row0);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              ptx::tma_gather4_2d_pair(dst + c * 2048 + i * 512, &tmap_k1, bar,
+                                       (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, q.r[0], q.r[1], q.r[2], q.r[3]);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ Q loads
+    if (lane == 0) {
+      SpaWalk w;
+      w.start(a.p, cluster);
+      bool ok = true;
+      const uint32_t bar = ptx::map_to_rank(q_full, 0);
+      for (uint32_t n = 0; w.more() && ok; ++n, w.next_job()) {
+        ok = ptx::mbar_wait(q_empty, (n & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        if (rank == 0) ptx::mbar_arrive_expect_tx(q_full, 2 * kSpaQBytes);
+#pragma unroll 1
+        for (int f = 0; f < 9; ++f)
+          ptx::tma_load_2d_pair(ptx::smem_u32(q_s) + f * kSpaQBlk, f < 8 ? &tmap_q : &tmap_qr, bar, f < 8 ? f * 64 : 0,
+                                w.j.row0 + (int32_t)rank * 64);
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ QK^T issuer
+    if (rank == 0 && lane == 0) {
+      SpaWalk w;
+      w.start(a.p, cluster);
+      bool ok = true;
+      const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
+      uint32_t n = 0;
+      for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
+        ok = ptx::mbar_spin(q_full, n_job & 1, abort_flag);
+        const int32_t stop = w.stop();
+        for (int32_t t = w.tile(); t < stop && ok; ++t, ++n) {
+          const uint32_t b = n & 1;
+          ok = ptx::mbar_spin_cluster(&s_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int f = 0; f < 9; ++f) {
+            ok = ok && ptx::mbar_spin(&k_full[f], n & 1, abort_flag);
+            if (!ok) break;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)   // (addresses in a descriptor count 16 bytes)
+              ptx::mma_ss_pair(tmem + kSpaTmS + b * 64, qd + (f * kSpaQBlk + kk * 32) / 16, kd + (f * kSpaBlk + kk * 32) / 16,
+                               a.idesc_qk, (f | kk) ? 1u : 0u);
+            ptx::mma_commit_pair(&k_empty[f]);
+          }
+          if (ok) ptx::mma_commit_pair(&s_full[b]);
+        }
+        if (ok) ptx::mma_commit_pair(q_empty);
+      }
+    }
+  } else if (warp == kSpaPvWarp) {
+    // ------------------------------------------------------------------ PV issuer
+    if (rank == 0 && lane == 0) {
+      SpaWalk w;
+      w.start(a.p, cluster);
+      bool ok = true;
+      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 2048, 1024);
+      uint32_t n = 0;
+      for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
+        ok = ptx::mbar_spin_cluster(o_free, (n_job & 1) ^ 1, abort_flag);
+        const int32_t first = w.tile(), stop = w.stop();
+        for (int32_t t = first; t < stop && ok; ++t, ++n) {
+          ok = ptx::mbar_spin_cluster(p_full, n & 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            ok = ok && ptx::mbar_spin(&v_full[g], n & 1, abort_flag);
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              ptx::mma_ss_pair(tmem + kSpaTmO + c * 128, pd + ((g >> 2) * kSpaPBlk + (g & 3) * 32) / 16,
+                               vd + (g * kSpaBlk + c * 4096) / 16, a.idesc_pv, (t > first || g > 0) ? 1u : 0u);
+            ptx::mma_commit_pair(&v_empty[g]);
+          }
+          if (ok) ptx::mma_commit_pair(p_empty);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax + epilogue
+    const int g = (warp - kSpaSoftWarp0) >> 2;    // takes keys 32 g .. 32 g + 31 of its half
+    const int quarter = warp & 3;
+    const int L = quarter * 32 + lane;            // tensor-memory lane
+    const int hl = L & 63, half = L >> 6;         // row of this CTA; half of N
+    const int trow = (int)rank * 64 + hl;         // row of the tile
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_empty_lead0 = ptx::map_to_rank(&s_empty[0], 0), s_empty_lead1 = ptx::map_to_rank(&s_empty[1], 0);
+    const uint32_t p_full_lead = ptx::map_to_rank(p_full, 0), o_free_lead = ptx::map_to_rank(o_free, 0);
+    uint64_t* xb = &x_bar[quarter & 1];
+    uint32_t n = 0, n_x = 0;
+    bool ok = true;
+    auto signal_lead = [&](uint64_t* local, uint32_t remote, bool publish) {
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) ptx::mbar_arrive(local);
+        else if (publish) ptx::mbar_arrive_remote_release(remote);
+        else ptx::mbar_arrive_remote_relaxed(remote, 0u);
+      }
+    };
+    // The values of the row's four threads (two buffers: a warp writes one of them again only after all four have arrived
+    // for the other, which they do after reading this one).
+    auto exchange = [&](float v, float4& all) -> bool {
+      float* x = xm + (n_x & 1) * 256;
+      x[(half * 2 + g) * 64 + hl] = v;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(xb);
+      const bool got = ptx::mbar_spin_warp(xb, n_x & 1, abort_flag);
+      all = make_float4(x[hl], x[64 + hl], x[128 + hl], x[192 + hl]);
+      ++n_x;
+      return got;
+    };
+    SpaWalk w;
+    w.start(a.p, cluster);
+    for (; w.more() && ok; w.next_job()) {
+      const SpaJob& j = w.j;
+      const int32_t first = w.tile(), stop = w.stop();
+      const int32_t slot = spa_slot(j, first, stop, cluster);
+      // positions that this thread's row sees
+      int32_t vis = 0;
+      if (trow < j.nrows) {
+        const int32_t tok = (j.head0 + trow) / a.p.n1;       // counted from the tile's first token
+        if (!j.packed) vis = a.p.seq.sparse_mode == 3 ? min(j.vis0 + tok, j.hi) : j.hi;
+        else {
+          const int32_t t = (j.row0 + trow) / a.p.n1;
+          const RowInfo ri = row_info(a.p.seq, t);
+          const SpaSeq s = spa_seq(a.p, ri.b, j.hi);
+          if (s.packed && t - s.start < s.act_q) vis = j.hi;
+        }
+      }
+      float m_ref = -INFINITY, m_true = -INFINITY, l = 0.f;
+      bool tainted = false;
+      for (int32_t t = first; t < stop && ok; ++t, ++n) {
+        const uint32_t b = n & 1;
+        ok = ptx::mbar_spin_warp(&s_full[b], (n >> 1) & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        float sc[32];
+        ptx::tmem_ld_x32(lane_addr + kSpaTmS + b * 64 + g * 32, reinterpret_cast<uint32_t*>(sc));
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        signal_lead(&s_empty[b], b ? s_empty_lead1 : s_empty_lead0, false);
+        const int32_t k0 = j.key0 + t * kSpaKeys + half * 64 + g * 32;    // position of sc[0]
+        if (__any_sync(0xffffffffu, k0 < j.lo || k0 + 32 > vis)) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const bool seen = k0 + k >= j.lo && k0 + k < vis;
+            // (a hidden key that another row of the tile sees)
+            if (!seen && k0 + k >= j.lo && k0 + k < j.hi && !(fabsf(sc[k]) < INFINITY)) tainted = true;
+            sc[k] = seen ? sc[k] * a.scale_log2 : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) sc[k] *= a.scale_log2;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          mx4[0] = fmaxf(mx4[0], sc[k]); mx4[1] = fmaxf(mx4[1], sc[k + 1]);
+          mx4[2] = fmaxf(mx4[2], sc[k + 2]); mx4[3] = fmaxf(mx4[3], sc[k + 3]);
+        }
+        float4 all;
+        ok = exchange(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), all);
+        if (!ok) break;
+        const float mx = fmaxf(fmaxf(all.x, all.y), fmaxf(all.z, all.w));
+        m_true = fmaxf(m_true, mx);
+        // the reference follows the maximum where it is exceeded by more than the guard (or where the row had none yet)
+        const bool raise = mx > m_ref + kSpaGuard || (m_ref == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float m_new = raise ? mx : m_ref;
+          const float f = raise ? (m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new)) : 1.f;
+          l *= f;
+          m_ref = m_new;
+          if (t > first) {
+            ok = ptx::mbar_spin_warp(p_empty, (n - 1) & 1, abort_flag);     // O is complete up to the tile before
+            if (!ok) break;
+            ptx::tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              const uint32_t at = lane_addr + kSpaTmO + g * 128 + c * 32;
+              ptx::tmem_ld_x32(at, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              ptx::tmem_st_x32(at, o);
+            }
+            ptx::tmem_st_wait();
+          }
+        }
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;       // (a row without a key yet: every sc is -inf, P = 0)
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pw[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float e0 = ex2(sc[k] - ref), e1 = ex2(sc[k + 1] - ref), e2 = ex2(sc[k + 2] - ref), e3 = ex2(sc[k + 3] - ref);
+          sum4[0] += e0; sum4[1] += e1; sum4[2] += e2; sum4[3] += e3;
+          pw[k / 2] = pack2(e0, e1, a.is_bf16);
+          pw[k / 2 + 1] = pack2(e2, e3, a.is_bf16);
+        }
+        l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        // P once the value products of the tile before have read theirs
+        ok = ptx::mbar_spin_warp(p_empty, (n & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        {
+          unsigned char* prow = p_s + half * kSpaPBlk + hl * 128;   // keys half * 64 .. are the first or second 64
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(prow + (((g * 4 + c) ^ (hl & 7)) << 4)) =
+                make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before();
+        signal_lead(p_full, p_full_lead, true);
+      }
+      if (!ok) break;
+      // ---- the row's sum, then O
+      float4 ls;
+      ok = exchange(l, ls);
+      if (!ok) break;
+      const float l_row = (ls.x + ls.y) + (ls.z + ls.w);
+      if (tainted && a.p.redo != nullptr) {
+        const int32_t tok = (j.row0 + trow) / a.p.n1;
+        if (trow < j.nrows && !j.packed && atomicExch(&a.p.redo[tok], 1) == 0) a.p.redo_list[atomicAdd(a.p.redo_count, 1)] = tok;
+      }
+      ok = ptx::mbar_spin_warp(p_empty, (n - 1) & 1, abort_flag);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const bool any = l_row != 0.f;                 // (a sum that is not a number stays one)
+      const float inv = any ? 1.f / l_row : 0.f;
+      const float total = any ? l_row * ex2(m_ref - m_true) : 0.f;     // relative to the row's maximum
+      const int32_t col0 = g * 256 + half * 128;     // this lane's columns
+      if (slot >= 0) {
+        float* o_row = a.p.part_o + ((int64_t)slot * kSpaRows + trow) * 512 + col0;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          ptx::tmem_ld_x32(lane_addr + kSpaTmO + g * 128 + c * 32, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+          if (any) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ptx::st_global_v8(o_row + c * 32 + i * 8, o + i * 8);
+          }
+        }
+        if (g == 0 && half == 0) {
+          a.p.part_m[(int64_t)slot * kSpaRows + trow] = m_true;
+          a.p.part_l[(int64_t)slot * kSpaRows + trow] = total;
+        }
+      } else {
+        unsigned char* o_row = (unsigned char*)a.p.out + (((int64_t)j.row0 + trow) * 512 + col0) * 2;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32], wd[16];
+          ptx::tmem_ld_x32(lane_addr + kSpaTmO + g * 128 + c * 32, o);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            wd[i] = any ? pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv, a.is_bf16) : 0u;
+          if (trow < j.nrows) {
+            ptx::st_global_v8(o_row + c * 64, wd);
+            ptx::st_global_v8(o_row + c * 64 + 32, wd + 8);
+          }
+        }
+        if (g == 0 && half == 0 && trow < j.nrows && a.p.softmax_max != nullptr) {
+          const bool give = a.p.return_lse && any;
+          a.p.softmax_max[(int64_t)j.row0 + trow] = give ? m_true * 0.6931471805599453f : 0.f;
+          a.p.softmax_sum[(int64_t)j.row0 + trow] = give ? total : 0.f;
+        }
+      }
+      ptx::tc_fence_before();
+      signal_lead(o_free, o_free_lead, false);
+    }
+  }
+
+  // ---------------------------------------------------------------------- teardown
+  __syncwarp();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);  // let copies / products in flight land
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  // neither CTA may leave while its peer can still signal it or run a pair product on its memory
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (warp == 2) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(a.p.status, misaligned ? 2 : 1);
+}
+
+// ---- join: a warp per (token, head) whose result is in parts, or that sees nothing ------------------
+constexpr int kSpaJoinWarps = 8;
+__global__ void __launch_bounds__(kSpaJoinWarps * 32) spa_join_kernel(const SpaDev p, int32_t is_bf16) {
+  grid_dep_launch();
+  grid_dep_wait();
+  const int lane = threadIdx.x & 31;
+  const int32_t tok = blockIdx.x, h = blockIdx.y * kSpaJoinWarps + (threadIdx.x >> 5);
+  if (h >= p.n1) return;
+  const SpaPlan w = *p.plan;
+  const RowInfo ri = row_info(p.seq, tok);
+  const SpaSeq s = spa_seq(p, ri.b, w.prefix);
+  const int64_t row = (int64_t)tok * p.n1 + h;
+  // parts of the row: tiles of its own job, then of the prefix job
+  int32_t first[2] = {0, 0}, count[2] = {0, 0}, uncut[2] = {-1, -1}, trow[2] = {0, 0};
+  if (tok - s.start < s.act_q) {
+    const int32_t r = (tok - s.start) * p.n1 + h;
+    int32_t place[2] = {p.prefix_tiles + spa_own_place(p, ri.b, s.start) + r / kSpaRows, (int32_t)(row / kSpaRows)};
+    trow[0] = r % kSpaRows;
+    trow[1] = (int32_t)(row % kSpaRows);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && !s.packed) continue;
+      const int32_t i = p.job_of[place[k]];
+      if (i < 0) continue;
+      const int32_t t0 = p.job[i].tile0, t1 = t0 + p.job[i].tiles - 1;
+      first[k] = t0 / w.share;
+      count[k] = t1 / w.share - first[k] + 1;
+      if (count[k] == 1) {
+        uncut[k] = p.job[i].slot;
+        if (uncut[k] < 0) return;        // the job wrote the row itself
+      }
+    }
+  }
+  const int32_t parts = count[0] + count[1];
+  // partial of part i: a job's first share leaves it at 2 c + 1, the later ones at 2 c
+  auto at = [&](int32_t i) -> int64_t {
+    const int k = i >= count[0];
+    if (k) i -= count[0];
+    const int32_t slot = count[k] == 1 ? uncut[k] : 2 * (first[k] + i) + (i == 0 ? 1 : 0);
+    return (int64_t)slot * kSpaRows + trow[k];
+  };
+  float mx = -INFINITY;
+  for (int32_t i = lane; i < parts; i += 32)
+    if (p.part_l[at(i)] != 0.f) mx = fmaxf(mx, p.part_m[at(i)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  float4 acc[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.f;
+  for (int32_t i0 = 0; i0 < parts; i0 += 32) {
+    float wt = 0.f;
+    if (i0 + lane < parts) {
+      const float l = p.part_l[at(i0 + lane)];
+      if (l != 0.f) wt = l * ex2(p.part_m[at(i0 + lane)] - mx);
+    }
+    for (int32_t i = i0; i < min(parts, i0 + 32); ++i) {
+      const float f = __shfl_sync(0xffffffffu, wt, i - i0);
+      if (f == 0.f) continue;            // (its O may never have been written)
+      den += f;
+      const float4* o = reinterpret_cast<const float4*>(p.part_o + at(i) * 512);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 v = o[c * 32 + lane];
+        acc[c].x += f * v.x; acc[c].y += f * v.y; acc[c].z += f * v.z; acc[c].w += f * v.w;
+      }
+    }
+  }
+  const bool any = den != 0.f;
+  const float inv = any ? 1.f / den : 0.f;
+  uint2* out = reinterpret_cast<uint2*>((unsigned char*)p.out + row * 1024);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    out[c * 32 + lane] = make_uint2(pack2(acc[c].x * inv, acc[c].y * inv, is_bf16), pack2(acc[c].z * inv, acc[c].w * inv, is_bf16));
+  if (lane == 0 && p.softmax_max != nullptr) {
+    const bool give = p.return_lse && any;
+    p.softmax_max[row] = give ? mx * 0.6931471805599453f : 0.f;
+    p.softmax_sum[row] = give ? den : 0.f;
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------------
+constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
+
+struct SpaWs {
+  size_t plan, job, job_of, first_job, redo, redo_list, redo_count, part_m, part_l, part_o, total;
+  int64_t prefix_tiles, own_tiles, own_tiles_per_seq, slots;
+  bool pack, redo_used;
+};
+inline SpaWs spa_ws_layout(const DsaSpaParams* p, int64_t rows) {
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  auto tiles = [](int64_t r) { return (r + kSpaRows - 1) / kSpaRows; };
+  SpaWs w;
+  const bool tnd = p->layout_q == DSA_LAYOUT_TND;
+  // packing needs a prefix and sequences of at most kSpaPackRows rows
+  w.pack = (p->prefix_device != nullptr || p->prefix >= kSpaPackKeys) && p->n1 <= kSpaPackRows;
+  w.prefix_tiles = w.pack ? tiles(rows * p->n1) : 0;
+  w.own_tiles_per_seq = tnd ? 0 : std::max<int64_t>(1, tiles((int64_t)p->s1 * p->n1));
+  w.own_tiles = tnd ? rows * p->n1 / kSpaRows + p->batch : p->batch * w.own_tiles_per_seq;
+  // a packed sequence has one tile of its own and touches two prefix tiles at most
+  w.slots = 2 * kSpaClusters + (w.pack ? std::min<int64_t>(w.own_tiles, p->batch) + std::min<int64_t>(w.prefix_tiles, 2ll * p->batch) : 0);
+  // rows of a tile see different keys only when it holds several tokens of a sequence under the causal mask
+  w.redo_used = p->sparse_mode == 3 && p->n1 % kSpaRows != 0 && (tnd || p->s1 > 1);
+  const size_t places = (size_t)(w.prefix_tiles + w.own_tiles);
+  w.plan = 0;
+  w.job = 256;
+  w.job_of = w.job + up(places * sizeof(SpaJob));
+  w.first_job = w.job_of + up(places * 4);
+  w.redo_count = w.first_job + up(kSpaClusters * 4);
+  w.redo = w.redo_count + 256;
+  w.redo_list = w.redo + (w.redo_used ? up((size_t)rows * 4) : 0);
+  w.part_m = w.redo_list + (w.redo_used ? up((size_t)rows * 4) : 0);
+  w.part_l = w.part_m + up((size_t)w.slots * kSpaRows * 4);
+  w.part_o = w.part_l + up((size_t)w.slots * kSpaRows * 4);
+  w.total = w.part_o + (size_t)w.slots * kSpaRows * 512 * 4;
+  return w;
+}
+
+inline bool spa_sm100_eligible(const DsaSpaParams* p, int64_t rows) {
+  if (((uintptr_t)p->query & 15u) || ((uintptr_t)p->query_rope & 15u) || ((uintptr_t)p->out & 31u)) return false;
+  if (p->key_rows >= 0x7FFFFFFF - 256 || rows < 1) return false;
+  const SpaWs w = spa_ws_layout(p, rows);
+  // tiles of all jobs are counted in 32 bits
+  const int64_t key_tiles = ((int64_t)p->max_blocks * p->block_size + kSpaKeys - 1) / kSpaKeys + 1;
+  return (w.prefix_tiles + w.own_tiles) * key_tiles < (1ll << 30);
+}
+
+// The first call on a device raises the kernels' shared-memory limits there.  Safe to call from several host threads.
+inline bool spa_sm100_prepare(int dev) {
+  static std::atomic<int> ready[64];
+  static std::mutex setup_lock;
+  if (dev < 0 || dev >= 64) return false;
+  if (ready[dev].load(std::memory_order_acquire)) return true;
+  std::lock_guard<std::mutex> g(setup_lock);
+  const int redo_smem = (kSfaSimtHeads + kSfaSimtKeys) * (512 + 64 + kSfaSimtPad) * 2;
+  if (cudaFuncSetAttribute(spa_fwd_sm100_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSpaSmemBytes) != cudaSuccess ||
+      cudaFuncSetAttribute(sfa_redo_kernel<__nv_bfloat16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, redo_smem) != cudaSuccess ||
+      cudaFuncSetAttribute(sfa_redo_kernel<__half, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, redo_smem) != cudaSuccess)
+    return false;
+  ready[dev].store(1, std::memory_order_release);
+  return true;
+}
+
+// `dense`: the call for the row-by-row kernel.
+inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t* status, void* scratch, cudaStream_t st) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return DSA_ERR_CUDA;
+  if (!spa_sm100_prepare(dev)) return DSA_ERR_CUDA;
+  const bool bf16 = p->dtype == DSA_DTYPE_BF16;
+  const SpaWs w = spa_ws_layout(p, dense.rows);
+  char* ws = (char*)scratch;
+  SpaArgs a;
+  SpaDev& d = a.p;
+  d.seq = dense.seq;
+  d.prefix_device = p->prefix_device; d.prefix = p->prefix;
+  d.rows = dense.rows; d.n1 = p->n1;
+  d.prefix_tiles = (int32_t)w.prefix_tiles; d.own_tiles = (int32_t)w.own_tiles; d.own_tiles_per_seq = (int32_t)w.own_tiles_per_seq;
+  d.pack_rows = w.pack ? kSpaPackRows : 0;
+  d.clusters = kSpaClusters;
+  d.plan = (SpaPlan*)(ws + w.plan); d.job = (SpaJob*)(ws + w.job); d.job_of = (int32_t*)(ws + w.job_of);
+  d.first_job = (int32_t*)(ws + w.first_job);
+  d.redo = w.redo_used ? (int32_t*)(ws + w.redo) : nullptr;
+  d.redo_list = (int32_t*)(ws + w.redo_list); d.redo_count = (int32_t*)(ws + w.redo_count);
+  d.status = status;
+  d.part_o = (float*)(ws + w.part_o); d.part_m = (float*)(ws + w.part_m); d.part_l = (float*)(ws + w.part_l);
+  d.out = p->out; d.softmax_max = p->softmax_max; d.softmax_sum = p->softmax_sum; d.return_lse = p->return_lse != 0;
+  a.idesc_qk = ptx::idesc_f16(bf16 ? 1u : 0u, 128, kSpaKeys, 0, 0);
+  a.idesc_pv = ptx::idesc_f16(bf16 ? 1u : 0u, 128, 256, 0, 1);
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.is_bf16 = bf16 ? 1 : 0;
+  a.key_rows = (int32_t)p->key_rows;
+  const uint64_t rows = (uint64_t)dense.rows * p->n1, keys = (uint64_t)p->key_rows;
+  CUtensorMap q, qr, k16, r16, k1, r1;
+  if (!make_tmap_2d_16bit(&q, p->query, rows, 512, 1024, 64, 64, bf16) ||
+      !make_tmap_2d_16bit(&qr, p->query_rope, rows, 64, 128, 64, 64, bf16) ||
+      !make_tmap_2d_16bit(&k16, p->key, keys, 512, 1024, 16, 64, bf16) ||
+      !make_tmap_2d_16bit(&r16, p->key_rope, keys, 64, 128, 16, 64, bf16) ||
+      !make_tmap_gather4_16bit(&k1, p->key, keys, 512, 1024, 64, bf16) ||
+      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16))
+    return DSA_ERR_CUDA;
+  if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
+  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, k16, r16, k1, r1, a) !=
+      cudaSuccess)
+    return DSA_ERR_CUDA;
+  if (launch_after(spa_join_kernel, dim3(d.rows, (p->n1 + kSpaJoinWarps - 1) / kSpaJoinWarps), dim3(kSpaJoinWarps * 32), 0, st, d,
+                   a.is_bf16) != cudaSuccess)
+    return DSA_ERR_CUDA;
+  count_launch(3);
+  if (w.redo_used) {
+    const size_t smem = (size_t)(kSfaSimtHeads + kSfaSimtKeys) * (p->d + p->d_rope + kSfaSimtPad) * 2;
+    const int64_t work = (int64_t)d.rows * ((p->n1 + kSfaSimtHeads - 1) / kSfaSimtHeads);
+    const dim3 grid((unsigned)std::min<int64_t>(work, 296));
+    const cudaError_t rc = bf16 ? launch_after(sfa_redo_kernel<__nv_bfloat16, true>, dim3(grid), dim3(kSfaSimtThreads), smem, st,
+                                               dense, d.redo_list, d.redo_count)
+                                : launch_after(sfa_redo_kernel<__half, true>, dim3(grid), dim3(kSfaSimtThreads), smem, st, dense,
+                                               d.redo_list, d.redo_count);
+    if (rc != cudaSuccess) return DSA_ERR_CUDA;
+    count_launch();
+  }
+  return DSA_OK;
+}
+
+}  // namespace dsa
