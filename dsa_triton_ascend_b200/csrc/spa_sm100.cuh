@@ -19,7 +19,8 @@
 // with A (64 rows a CTA) in shared memory takes 16 + N / 4 cycles per 16 of K: 36 x 48 + 16 x 80 = 3008 cycles for a tile
 // of 128 keys, against 2176 at the full rate and 3584 as two tiles of 64.
 // Tensor memory: lanes 0..63 hold a CTA's rows with the first half of N, lanes 64..127 the same rows with the second:
-// S buffers 2 x 64 columns, O 256.
+// O 256 columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off, so that a score is too small by
+// 5e-7 of itself after 36 steps, and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
 //
 // Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, 16 of them per box where the page size is a
 // multiple of 16, else (and at the ends of a range, where some of 16 are not wanted) with gather4, four rows each; rows
@@ -35,7 +36,7 @@
 // 0 x infinity would be NaN: a hidden key whose score is not finite (every non-finite latent makes it so, for every row)
 // marks the token, and sfa_redo_kernel computes it again from its visible keys alone.  Normally no token.
 //
-// Warps (416 threads): 0 K loads, 1 V loads, 2 Q loads and tensor memory, 3 QK issuer, 4..11 softmax, 12 PV issuer.
+// Warps (448 threads): 0 K loads, 1 V loads, 2 Q loads and tensor memory, 3 and 13 QK issuers, 4..11 softmax, 12 PV issuer.
 // All waits are bounded; one that gives up sets the status word.
 #pragma once
 
@@ -51,20 +52,22 @@ namespace dsa {
 
 constexpr int kSpaRows = 128;        // rows per tile (64 per CTA)
 constexpr int kSpaKeys = 128;        // keys per tile
-constexpr int kSpaThreads = 416;
-constexpr int kSpaSoftWarp0 = 4, kSpaPvWarp = 12;
+constexpr int kSpaThreads = 512;
+constexpr int kSpaQkWarp0 = 3, kSpaSoftWarp0 = 4, kSpaPvWarp = 12, kSpaQkWarp1 = 13, kSpaKWarp1 = 14, kSpaVWarp1 = 15;
 constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
 constexpr int kSpaPackKeys = 256;    // a shorter prefix is not worth the partials
 constexpr int kSpaPlanThreads = 1024;
 
 constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
 constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
-constexpr uint32_t kSpaBlk = 8192;                          // a K block (64 keys x 64 features) or V block (16 keys x 256 columns)
+constexpr uint32_t kSpaBlk = 64 * 128;                      // 64 keys x 64 features
+constexpr uint32_t kSpaKUnit = 2 * kSpaBlk;                 // two such blocks; the fifth unit, the rope, is one
+constexpr uint32_t kSpaVUnit = 4 * 32 * 128;                // 32 keys x four blocks of 64 columns
 constexpr uint32_t kSpaPBlk = 64 * 128;                     // 64 rows x 64 keys
 constexpr uint32_t kSpaOffQ = 0;
 constexpr uint32_t kSpaOffK = kSpaOffQ + kSpaQBytes;
 constexpr uint32_t kSpaOffV = kSpaOffK + 9 * kSpaBlk;
-constexpr uint32_t kSpaOffP = kSpaOffV + 8 * kSpaBlk;
+constexpr uint32_t kSpaOffP = kSpaOffV + 4 * kSpaVUnit;
 constexpr uint32_t kSpaOffX = kSpaOffP + 2 * kSpaPBlk;      // float [2][4][64]
 constexpr uint32_t kSpaOffBar = kSpaOffX + 2048;
 constexpr uint32_t kSpaSmemBytes = kSpaOffBar + 512;
@@ -331,38 +334,41 @@ struct SpaArgs {
   SpaDev p;
   uint32_t idesc_qk, idesc_pv;
   float scale_log2;
-  int32_t is_bf16, key_rows;
+  int32_t is_bf16, key_rows, blocks;
+  uint32_t page_mul, page_shift;   // position / page size = position * page_mul >> page_shift (positions below 2^31)
 };
 
-// The four rows of the cache at positions pos .. pos + 3 of a job (key_rows, past the tensor: zeros).
-struct SpaQuad { int32_t r[4]; bool box; };
-__device__ __forceinline__ SpaQuad spa_quad(const SpaArgs& a, const SpaJob& j, int32_t pos) {
-  const int32_t bs = a.p.seq.block_size;
-  const int32_t* table = a.p.seq.block_table + (int64_t)j.table_row * a.p.seq.max_blocks;
-  const int32_t blocks = a.key_rows / bs;
-  SpaQuad q;
-  const int32_t first = pos & ~15;
-  const bool whole = (bs & 15) == 0;
-  q.box = whole && first >= j.lo && first + 16 <= j.hi;
-  int32_t page = -1, blk = -1;
+// Where the positions pos .. pos + 3 of a job (pos a multiple of 4) lie in the cache: the look-ups first, so that they are
+// in flight over the waits of the tile before, the rows when they are needed.  A position that is not
+// wanted (outside lo .. hi - 1) or whose block is absent gets key_rows, a row past the tensor, which is loaded as zeros.
+struct SpaQuad {
+  int32_t blk[4], off[4];
+  __device__ __forceinline__ void look_up(const SpaArgs& a, const SpaJob& j, int32_t pos) {
+    const int32_t* table = a.p.seq.block_table + (int64_t)j.table_row * a.p.seq.max_blocks;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t x = pos + i;
-    q.r[i] = a.key_rows;
-    if (x >= j.lo && x < j.hi) {
-      const int32_t g = x / bs;
-      if (g != page) { page = g; blk = table[g]; }
-      if (blk >= 0 && blk < blocks) q.r[i] = blk * bs + (x - g * bs);
+    for (int i = 0; i < 4; ++i) {
+      const int32_t x = pos + i;
+      const bool in = x >= j.lo && x < j.hi;
+      const int32_t page = (int32_t)(((uint64_t)(uint32_t)x * a.page_mul) >> a.page_shift);
+      off[i] = in ? x - page * a.p.seq.block_size : -1;
+      blk[i] = in ? table[page] : -1;
     }
   }
-  return q;
+  __device__ __forceinline__ int32_t row(const SpaArgs& a, int i) const {
+    return blk[i] >= 0 && blk[i] < a.blocks ? blk[i] * a.p.seq.block_size + off[i] : a.key_rows;
+  }
+};
+// Are n positions from pos on (a multiple of n) one box of rows: in one page and all wanted, or none of them wanted?
+__device__ __forceinline__ bool spa_box(const SpaArgs& a, const SpaJob& j, int32_t pos, int32_t n) {
+  return pos + n <= j.lo || pos >= j.hi || ((a.p.seq.block_size & (n - 1)) == 0 && pos >= j.lo && pos + n <= j.hi);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSpaThreads, 1)
 spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_qr,
+                     const __grid_constant__ CUtensorMap tmap_k64, const __grid_constant__ CUtensorMap tmap_r64,
                      const __grid_constant__ CUtensorMap tmap_k16, const __grid_constant__ CUtensorMap tmap_r16,
                      const __grid_constant__ CUtensorMap tmap_k1, const __grid_constant__ CUtensorMap tmap_r1,
-                     const SpaArgs a) {
+                     const __grid_constant__ CUtensorMap tmap_v32, const SpaArgs a) {
   extern __shared__ __align__(1024) unsigned char spa_sm[];
   unsigned char* q_s = spa_sm + kSpaOffQ;
   unsigned char* k_s = spa_sm + kSpaOffK;
@@ -370,13 +376,13 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   unsigned char* p_s = spa_sm + kSpaOffP;
   float* xm = reinterpret_cast<float*>(spa_sm + kSpaOffX);      // [2 turns][4 threads of a row][64 rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(spa_sm + kSpaOffBar);
-  uint64_t* k_full = bars;         // [9] even CTA: both CTAs' blocks have landed (bytes)
-  uint64_t* k_empty = bars + 9;    // [9] the products that read the block are done (commit, both CTAs)
-  uint64_t* v_full = bars + 18;    // [8]
-  uint64_t* v_empty = bars + 26;   // [8]
+  uint64_t* k_full = bars;         // [5] even CTA: both CTAs' parts of the unit have landed (bytes)
+  uint64_t* k_empty = bars + 5;    // [5] the products that read the unit are done (commit, both CTAs)
+  uint64_t* v_full = bars + 10;    // [4]
+  uint64_t* v_empty = bars + 14;   // [4]
   uint64_t* q_full = bars + 34;    // even CTA: both CTAs' rows have landed
-  uint64_t* q_empty = bars + 35;   // the job's last score product is done (commit, both CTAs)
-  uint64_t* s_full = bars + 36;    // [2] scores of a tile are done (commit, both CTAs)
+  uint64_t* q_empty = bars + 35;   // the job's last score products are done (commit of both issuers, both CTAs)
+  uint64_t* s_full = bars + 36;    // [2] scores of a tile are done (commit of both issuers, both CTAs)
   uint64_t* s_empty = bars + 38;   // [2] even CTA: the softmax warps of both CTAs hold them in registers
   uint64_t* p_full = bars + 40;    // even CTA: P stored in both CTAs, O rescaled where it had to be
   uint64_t* p_empty = bars + 41;   // the tile's value products are done (commit, both CTAs)
@@ -392,12 +398,12 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 
   const bool misaligned = (ptx::smem_u32(spa_sm) & 1023u) != 0;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 9; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < 8; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
+    for (int i = 0; i < 5; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < 4; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
     ptx::mbar_init(q_full, 1);
-    ptx::mbar_init(q_empty, 1);
+    ptx::mbar_init(q_empty, 2);
     for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&s_empty[i], 16); ptx::mbar_init(&x_bar[i], 4);
+      ptx::mbar_init(&s_full[i], 2); ptx::mbar_init(&s_empty[i], 16); ptx::mbar_init(&x_bar[i], 4);
     }
     ptx::mbar_init(p_full, 16);
     ptx::mbar_init(p_empty, 1);
@@ -420,70 +426,118 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 
   if (*abort_flag) {
     // nothing started
-  } else if (warp == 0) {
+  } else if (warp == 0 || warp == kSpaKWarp1) {
     // ------------------------------------------------------------------ K loads
-    // Lane 4 g + i of the first 16 holds positions 16 g + 4 i .. + 3 of this CTA's 64; a group of 16 is one box per block.
-    const uint32_t dst0 = ptx::smem_u32(k_s) + (lane >> 2) * 2048;
+    // Two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3.  Lane 4 g + i of the first 16 holds positions
+    // 16 g + 4 i .. + 3 of this CTA's 64.  A unit is one box where the 64 lie in one page, else a box or four gathers per
+    // 16 keys and 64 features.  One lane issues: lanes that each issue their own cost 130 cycles a load.
+    const uint32_t dst0 = ptx::smem_u32(k_s), bar0 = ptx::map_to_rank(&k_full[0], 0);
+    const int u0 = warp == 0 ? 0 : 2, units = warp == 0 ? 3 : 2;
     SpaWalk w;
     w.start(a.p, cluster);
-    SpaQuad cur = {};
-    auto quad = [&](const SpaWalk& x) {
-      if (x.more() && lane < 16) cur = spa_quad(a, x.j, x.j.key0 + x.tile() * kSpaKeys + (int32_t)rank * 64 + lane * 4);
+    SpaQuad quad;
+    bool box64 = false, box16 = false;
+    auto look_up = [&]() {
+      if (!w.more()) return;
+      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64;
+      box64 = spa_box(a, w.j, pos, 64);
+      box16 = spa_box(a, w.j, pos + (lane & ~3) * 4, 16);
+      quad.look_up(a, w.j, pos + (lane & 15) * 4);
     };
-    quad(w);
+    look_up();
     bool ok = true;
     for (uint32_t n = 0; w.more() && ok; ++n) {
-      const SpaQuad q = cur;
+      int32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
+      const bool one = box64;
+      const uint32_t boxes = __ballot_sync(0xffffffffu, box16);
       w.next_tile();
-      quad(w);              // (the look-ups of the next tile are in flight while this one is waited for)
+      look_up();
 #pragma unroll 1
-      for (int f = 0; f < 9 && ok; ++f) {
-        ok = ptx::mbar_spin_warp(&k_empty[f], (n & 1) ^ 1, abort_flag);
+      for (int i = 0; i < units; ++i) {
+        const int u = i == 2 ? 4 : u0 + i;
+        ok = ptx::mbar_spin_warp(&k_empty[u], (n & 1) ^ 1, abort_flag);
         if (!ok) break;
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[f], 2 * kSpaBlk);
-        const uint32_t bar = ptx::map_to_rank(&k_full[f], 0);
-        const uint32_t dst = dst0 + f * kSpaBlk;
-        const int32_t x = f < 8 ? f * 64 : 0;
-        if (lane < 16) {
-          if (!q.box) ptx::tma_gather4_2d_pair(dst + (lane & 3) * 512, f < 8 ? &tmap_k1 : &tmap_r1, bar, x, q.r[0], q.r[1], q.r[2], q.r[3]);
-          else if ((lane & 3) == 0) ptx::tma_load_2d_pair(dst, f < 8 ? &tmap_k16 : &tmap_r16, bar, x, q.r[0]);
+        const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaKUnit;
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[u], u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
+        if (one) {
+          if (lane == 0) {
+            if (u < 4) ptx::tma_load_3d_pair(dst, &tmap_k64, bar, 0, r[0], u * 2);
+            else ptx::tma_load_2d_pair(dst, &tmap_r64, bar, 0, r[0]);
+          }
+        } else {
+#pragma unroll 1
+          for (int q = 0; q < 16; ++q) {
+            const int32_t y0 = __shfl_sync(0xffffffffu, r[0], q), y1 = __shfl_sync(0xffffffffu, r[1], q),
+                          y2 = __shfl_sync(0xffffffffu, r[2], q), y3 = __shfl_sync(0xffffffffu, r[3], q);
+            const bool box = (boxes >> q) & 1;
+            if (lane == 0) {
+#pragma unroll 1
+              for (int e = 0; e < (u < 4 ? 2 : 1); ++e) {
+                const uint32_t at = dst + e * kSpaBlk + q * 512;
+                const int32_t x = u < 4 ? u * 128 + e * 64 : 0;
+                if (box) ptx::tma_load_2d_pair(at, u < 4 ? &tmap_k16 : &tmap_r16, bar, x, y0);
+                else ptx::tma_gather4_2d_pair(at, u < 4 ? &tmap_k1 : &tmap_r1, bar, x, y0, y1, y2, y3);
+              }
+            }
+            if (box) q += 3;
+          }
         }
         __syncwarp();
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == kSpaVWarp1) {
     // ------------------------------------------------------------------ V loads
-    // Lane 4 g + i holds positions 16 g + 4 i .. + 3 of the tile's 128; group g is block g of the ring, and where it is
-    // whole pages' rows, lane i of it loads its column block i.
+    // Two warps, 1 has the units (32 keys x 256 columns) 0 and 2, 15 the units 1 and 3.  Lane 4 g + i holds positions
+    // 16 g + 4 i .. + 3 of the tile's 128.  A unit is one box, or a box or four gathers per 16 keys and 64 columns.
+    const uint32_t dst0 = ptx::smem_u32(v_s), bar0 = ptx::map_to_rank(&v_full[0], 0);
     SpaWalk w;
     w.start(a.p, cluster);
-    SpaQuad cur = {};
-    auto quad = [&](const SpaWalk& x) {
-      if (x.more()) cur = spa_quad(a, x.j, x.j.key0 + x.tile() * kSpaKeys + lane * 4);
+    SpaQuad quad;
+    bool box32 = false, box16 = false;
+    auto look_up = [&]() {
+      if (!w.more()) return;
+      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys;
+      box32 = spa_box(a, w.j, pos + (lane & ~7) * 4, 32);
+      box16 = spa_box(a, w.j, pos + (lane & ~3) * 4, 16);
+      quad.look_up(a, w.j, pos + lane * 4);
     };
-    quad(w);
+    look_up();
     bool ok = true;
     for (uint32_t n = 0; w.more() && ok; ++n) {
-      const SpaQuad q = cur;
-      w.next_tile();
-      quad(w);
-      const int32_t row0 = __shfl_sync(0xffffffffu, q.r[0], lane & ~3);
-#pragma unroll 1
-      for (int g = 0; g < 8 && ok; ++g) {
-        ok = ptx::mbar_spin_warp(&v_empty[g], (n & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[g], 2 * kSpaBlk);
-        const uint32_t bar = ptx::map_to_rank(&v_full[g], 0);
-        if ((lane >> 2) == g) {
-          const uint32_t dst = ptx::smem_u32(v_s) + g * kSpaBlk;
-          const int i = lane & 3;
-          if (q.box) {
-            ptx::tma_load_2d_pair(dst + i * 2048, &tmap_k16, bar, (i >> 1) * 256 + (int32_t)rank * 128 + (i & 1) * 64, row0);
-          } else {
+      int32_t r[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              ptx::tma_gather4_2d_pair(dst + c * 2048 + i * 512, &tmap_k1, bar,
-                                       (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, q.r[0], q.r[1], q.r[2], q.r[3]);
+      for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
+      const uint32_t wide = __ballot_sync(0xffffffffu, box32), boxes = __ballot_sync(0xffffffffu, box16);
+      w.next_tile();
+      look_up();
+#pragma unroll 1
+      for (int u = warp == 1 ? 0 : 1; u < 4; u += 2) {
+        ok = ptx::mbar_spin_warp(&v_empty[u], (n & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaVUnit;
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[u], 2 * kSpaVUnit);
+        if ((wide >> (u * 8)) & 1) {
+          const int32_t y = __shfl_sync(0xffffffffu, r[0], u * 8);
+          if (lane == 0) ptx::tma_load_5d_pair(dst, &tmap_v32, bar, 0, y, 0, 0, (int32_t)rank);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const int q = u * 8 + i;
+            const int32_t y0 = __shfl_sync(0xffffffffu, r[0], q), y1 = __shfl_sync(0xffffffffu, r[1], q),
+                          y2 = __shfl_sync(0xffffffffu, r[2], q), y3 = __shfl_sync(0xffffffffu, r[3], q);
+            const bool box = (boxes >> q) & 1;
+            if (lane == 0) {
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                const uint32_t at = dst + c * 4096 + i * 512;
+                const int32_t x = (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64;
+                if (box) ptx::tma_load_2d_pair(at, &tmap_k16, bar, x, y0);
+                else ptx::tma_gather4_2d_pair(at, &tmap_k1, bar, x, y0, y1, y2, y3);
+              }
+            }
+            if (box) i += 3;
           }
         }
         __syncwarp();
@@ -506,63 +560,82 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                                 w.j.row0 + (int32_t)rank * 64);
       }
     }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------------ QK^T issuer
-    if (rank == 0 && lane == 0) {
+  } else if (warp == kSpaQkWarp0 || warp == kSpaQkWarp1) {
+    // ------------------------------------------------------------------ QK^T issuers
+    // Two, each with its feature blocks and its partial score.  The loop is warp-uniform, one elected lane issues.
+    if (rank == 0) {
+      const bool second = warp == kSpaQkWarp1;      // units 2 and 3; the first: 0, 1 and the rope
+      const int units = second ? 2 : 3;
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
       const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
+      const uint32_t q_hi = (uint32_t)(qd >> 32), k_hi = (uint32_t)(kd >> 32);
+      const uint32_t tm = tmem + kSpaTmS + (second ? 64 : 0);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
-        ok = ptx::mbar_spin(q_full, n_job & 1, abort_flag);
+        ok = ptx::mbar_spin_warp(q_full, n_job & 1, abort_flag);
         const int32_t stop = w.stop();
         for (int32_t t = w.tile(); t < stop && ok; ++t, ++n) {
           const uint32_t b = n & 1;
-          ok = ptx::mbar_spin_cluster(&s_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
+          ok = ptx::mbar_spin_cluster_warp(&s_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
-#pragma unroll
-          for (int f = 0; f < 9; ++f) {
-            ok = ok && ptx::mbar_spin(&k_full[f], n & 1, abort_flag);
+#pragma unroll 1
+          for (int i = 0; i < units; ++i) {
+            const int u = second ? 2 + i : (i == 2 ? 4 : i);
+            ok = ptx::mbar_spin_warp(&k_full[u], n & 1, abort_flag);
             if (!ok) break;
+            if (ptx::elect_one()) {
+              const uint32_t ql = (uint32_t)qd + u * (2 * kSpaQBlk / 16), kl = (uint32_t)kd + u * (kSpaKUnit / 16);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)   // (addresses in a descriptor count 16 bytes)
-              ptx::mma_ss_pair(tmem + kSpaTmS + b * 64, qd + (f * kSpaQBlk + kk * 32) / 16, kd + (f * kSpaBlk + kk * 32) / 16,
-                               a.idesc_qk, (f | kk) ? 1u : 0u);
-            ptx::mma_commit_pair(&k_empty[f]);
+              for (int kk = 0; kk < 8; ++kk)   // (addresses in a descriptor count 16 bytes)
+                if (kk < 4 || u < 4)
+                  ptx::mma_ss_pair_lo(tm + b * 128, ql + (kk >> 2) * (kSpaQBlk / 16) + (kk & 3) * 2, q_hi,
+                                      kl + (kk >> 2) * (kSpaBlk / 16) + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
+              ptx::mma_commit_pair(&k_empty[u]);
+              if (i == units - 1) ptx::mma_commit_pair(&s_full[b]);
+            }
+            __syncwarp();
           }
-          if (ok) ptx::mma_commit_pair(&s_full[b]);
         }
-        if (ok) ptx::mma_commit_pair(q_empty);
+        if (ok && ptx::elect_one()) ptx::mma_commit_pair(q_empty);
+        __syncwarp();
       }
     }
   } else if (warp == kSpaPvWarp) {
     // ------------------------------------------------------------------ PV issuer
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
-      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 2048, 1024);
+      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 4096, 1024);
+      const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
-        ok = ptx::mbar_spin_cluster(o_free, (n_job & 1) ^ 1, abort_flag);
+        ok = ptx::mbar_spin_cluster_warp(o_free, (n_job & 1) ^ 1, abort_flag);
         const int32_t first = w.tile(), stop = w.stop();
         for (int32_t t = first; t < stop && ok; ++t, ++n) {
-          ok = ptx::mbar_spin_cluster(p_full, n & 1, abort_flag);
+          ok = ptx::mbar_spin_cluster_warp(p_full, n & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            ok = ok && ptx::mbar_spin(&v_full[g], n & 1, abort_flag);
+#pragma unroll 1
+          for (int u = 0; u < 4; ++u) {
+            ok = ptx::mbar_spin_warp(&v_full[u], n & 1, abort_flag);
             if (!ok) break;
+            if (ptx::elect_one()) {
+              const uint32_t pl = (uint32_t)pd + (u >> 1) * (kSpaPBlk / 16) + (u & 1) * 4, vl = (uint32_t)vd + u * (kSpaVUnit / 16);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-              ptx::mma_ss_pair(tmem + kSpaTmO + c * 128, pd + ((g >> 2) * kSpaPBlk + (g & 3) * 32) / 16,
-                               vd + (g * kSpaBlk + c * 4096) / 16, a.idesc_pv, (t > first || g > 0) ? 1u : 0u);
-            ptx::mma_commit_pair(&v_empty[g]);
+              for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (8192 / 16) + kk * (2048 / 16), v_hi,
+                                      a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
+              ptx::mma_commit_pair(&v_empty[u]);
+              if (u == 3) ptx::mma_commit_pair(p_empty);
+            }
+            __syncwarp();
           }
-          if (ok) ptx::mma_commit_pair(p_empty);
         }
       }
     }
@@ -625,8 +698,14 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         ptx::tc_fence_after();
         float sc[32];
-        ptx::tmem_ld_x32(lane_addr + kSpaTmS + b * 64 + g * 32, reinterpret_cast<uint32_t*>(sc));
-        ptx::tmem_ld_wait();
+        {
+          float s1[32];
+          ptx::tmem_ld_x32(lane_addr + kSpaTmS + b * 128 + g * 32, reinterpret_cast<uint32_t*>(sc));
+          ptx::tmem_ld_x32(lane_addr + kSpaTmS + b * 128 + 64 + g * 32, reinterpret_cast<uint32_t*>(s1));
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) sc[k] += s1[k];
+        }
         ptx::tc_fence_before();
         signal_lead(&s_empty[b], b ? s_empty_lead1 : s_empty_lead0, false);
         const int32_t k0 = j.key0 + t * kSpaKeys + half * 64 + g * 32;    // position of sc[0]
@@ -923,6 +1002,32 @@ inline bool spa_sm100_prepare(int dev) {
   return true;
 }
 
+// The latent cache [keys, 512] as [block 8][keys][64 features].  A box of 64 keys x two blocks is a K unit.
+inline bool spa_tmap_k(CUtensorMap* m, const void* base, uint64_t keys, bool bf16) {
+  EncodeTiledFn enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[3] = {64, keys, 8};
+  cuuint64_t strides[2] = {1024, 128};
+  cuuint32_t box[3] = {64, 64, 2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// The latent cache [keys, 512] as [rank 2][half 2][block 2][keys][64 columns]: column 256 half + 128 rank + 64 block.  A box of
+// 32 keys x both blocks x both halves is a V unit, 64-column blocks of 32 rows one behind the other.
+inline bool spa_tmap_v(CUtensorMap* m, const void* base, uint64_t keys, bool bf16) {
+  EncodeTiledFn enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  cuuint64_t dims[5] = {64, keys, 2, 2, 2};
+  cuuint64_t strides[4] = {1024, 128, 512, 256};
+  cuuint32_t box[5] = {64, 32, 2, 2, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims,
+             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // `dense`: the call for the row-by-row kernel.
 inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t* status, void* scratch, cudaStream_t st) {
   int dev = 0;
@@ -951,17 +1056,26 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.is_bf16 = bf16 ? 1 : 0;
   a.key_rows = (int32_t)p->key_rows;
+  a.blocks = (int32_t)(p->key_rows / p->block_size);
+  // mul = ceil(2^(31 + l) / size) with 2^l >= size: the error is below 2^31 size / 2^(31 + l) <= 1 step of the quotient
+  uint32_t l = 0;
+  while ((1ll << l) < p->block_size) ++l;
+  a.page_shift = 31 + l;
+  a.page_mul = (uint32_t)(((1ull << (31 + l)) + p->block_size - 1) / (uint64_t)p->block_size);
   const uint64_t rows = (uint64_t)dense.rows * p->n1, keys = (uint64_t)p->key_rows;
-  CUtensorMap q, qr, k16, r16, k1, r1;
+  CUtensorMap q, qr, k64, r64, k16, r16, k1, r1, v32;
   if (!make_tmap_2d_16bit(&q, p->query, rows, 512, 1024, 64, 64, bf16) ||
       !make_tmap_2d_16bit(&qr, p->query_rope, rows, 64, 128, 64, 64, bf16) ||
+      !spa_tmap_k(&k64, p->key, keys, bf16) ||
+      !make_tmap_2d_16bit(&r64, p->key_rope, keys, 64, 128, 64, 64, bf16) ||
       !make_tmap_2d_16bit(&k16, p->key, keys, 512, 1024, 16, 64, bf16) ||
       !make_tmap_2d_16bit(&r16, p->key_rope, keys, 64, 128, 16, 64, bf16) ||
       !make_tmap_gather4_16bit(&k1, p->key, keys, 512, 1024, 64, bf16) ||
-      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16))
+      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16) || !spa_tmap_v(&v32, p->key, keys, bf16))
     return DSA_ERR_CUDA;
   if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
-  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, k16, r16, k1, r1, a) !=
+  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, k64, r64, k16, r16,
+                   k1, r1, v32, a) !=
       cudaSuccess)
     return DSA_ERR_CUDA;
   if (launch_after(spa_join_kernel, dim3(d.rows, (p->n1 + kSpaJoinWarps - 1) / kSpaJoinWarps), dim3(kSpaJoinWarps * 32), 0, st, d,
