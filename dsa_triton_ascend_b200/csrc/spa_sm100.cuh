@@ -26,8 +26,8 @@
 // multiple of 16, else (and at the ends of a range, where some of 16 are not wanted) with gather4, four rows each; rows
 // that are not wanted and absent pages are read at a row past the tensor, which gives zeros without touching
 // memory: what lies behind a sequence's end never enters a product.  Bytes are counted on the even CTA's barriers, where
-// the products are issued.  Rings: K 9 blocks of 64 keys x 64 features, V 8 blocks of 16 keys x 256 columns, each of one
-// tile, refilled block by block.
+// the products are issued.  Rings: K five units of 64 keys x 128 features (the fifth, the rope, 64), one tile,
+// V three units of 32 keys x 256 columns, refilled unit by unit; P has two buffers.
 //
 // Softmax.  Eight warps take every tile together: the four threads of a row (two halves of N x two groups of 32 keys)
 // exchange their maxima through shared memory.  P is relative to a running reference that follows the maximum only when it is
@@ -64,11 +64,13 @@ constexpr uint32_t kSpaBlk = 64 * 128;                      // 64 keys x 64 feat
 constexpr uint32_t kSpaKUnit = 2 * kSpaBlk;                 // two such blocks; the fifth unit, the rope, is one
 constexpr uint32_t kSpaVUnit = 4 * 32 * 128;                // 32 keys x four blocks of 64 columns
 constexpr uint32_t kSpaPBlk = 64 * 128;                     // 64 rows x 64 keys
+constexpr uint32_t kSpaPBuf = 2 * kSpaPBlk;
+constexpr uint32_t kSpaVUnits = 3;                          // units in the ring (a tile has four)
 constexpr uint32_t kSpaOffQ = 0;
 constexpr uint32_t kSpaOffK = kSpaOffQ + kSpaQBytes;
 constexpr uint32_t kSpaOffV = kSpaOffK + 9 * kSpaBlk;
-constexpr uint32_t kSpaOffP = kSpaOffV + 4 * kSpaVUnit;
-constexpr uint32_t kSpaOffX = kSpaOffP + 2 * kSpaPBlk;      // float [2][4][64]
+constexpr uint32_t kSpaOffP = kSpaOffV + kSpaVUnits * kSpaVUnit;
+constexpr uint32_t kSpaOffX = kSpaOffP + 2 * kSpaPBuf;      // float [2][4][64]
 constexpr uint32_t kSpaOffBar = kSpaOffX + 2048;
 constexpr uint32_t kSpaSmemBytes = kSpaOffBar + 512;
 static_assert(kSpaSmemBytes <= 232448, "shared memory");
@@ -378,19 +380,19 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   uint64_t* bars = reinterpret_cast<uint64_t*>(spa_sm + kSpaOffBar);
   uint64_t* k_full = bars;         // [5] even CTA: both CTAs' parts of the unit have landed (bytes)
   uint64_t* k_empty = bars + 5;    // [5] the products that read the unit are done (commit, both CTAs)
-  uint64_t* v_full = bars + 10;    // [4]
-  uint64_t* v_empty = bars + 14;   // [4]
-  uint64_t* q_full = bars + 34;    // even CTA: both CTAs' rows have landed
-  uint64_t* q_empty = bars + 35;   // the job's last score products are done (commit of both issuers, both CTAs)
-  uint64_t* s_full = bars + 36;    // [2] scores of a tile are done (commit of both issuers, both CTAs)
-  uint64_t* s_empty = bars + 38;   // [2] even CTA: the softmax warps of both CTAs hold them in registers
-  uint64_t* p_full = bars + 40;    // even CTA: P stored in both CTAs, O rescaled where it had to be
-  uint64_t* p_empty = bars + 41;   // the tile's value products are done (commit, both CTAs)
-  uint64_t* o_free = bars + 42;    // even CTA: the softmax warps of both CTAs have read O
-  uint64_t* x_bar = bars + 43;     // [2] xm written: the four warps that hold the same 32 rows
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 45);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 46);
-  static_assert(47 * 8 <= 512, "barrier area");
+  uint64_t* v_full = bars + 10;    // [3] (ring)
+  uint64_t* v_empty = bars + 13;   // [3]
+  uint64_t* q_full = bars + 20;    // even CTA: both CTAs' rows have landed
+  uint64_t* q_empty = bars + 21;   // the job's last score products are done (commit of both issuers, both CTAs)
+  uint64_t* s_full = bars + 22;    // [2] scores of a tile are done (commit of both issuers, both CTAs)
+  uint64_t* s_empty = bars + 24;   // [2] even CTA: the softmax warps of both CTAs hold them in registers
+  uint64_t* p_full = bars + 16;    // [2] even CTA: P stored in both CTAs, O rescaled where it had to be
+  uint64_t* p_empty = bars + 18;   // [2] the tile's value products are done (commit, both CTAs)
+  uint64_t* o_free = bars + 26;    // even CTA: the softmax warps of both CTAs have read O
+  uint64_t* x_bar = bars + 27;     // [2] xm written: the four warps that hold the same 32 rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 30);
+  static_assert(31 * 8 <= 512, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_ctarank();
@@ -399,14 +401,13 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const bool misaligned = (ptx::smem_u32(spa_sm) & 1023u) != 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) { ptx::mbar_init(&k_full[i], 1); ptx::mbar_init(&k_empty[i], 1); }
-    for (int i = 0; i < 4; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
+    for (uint32_t i = 0; i < kSpaVUnits; ++i) { ptx::mbar_init(&v_full[i], 1); ptx::mbar_init(&v_empty[i], 1); }
     ptx::mbar_init(q_full, 1);
     ptx::mbar_init(q_empty, 2);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&s_full[i], 2); ptx::mbar_init(&s_empty[i], 16); ptx::mbar_init(&x_bar[i], 4);
     }
-    ptx::mbar_init(p_full, 16);
-    ptx::mbar_init(p_empty, 1);
+    for (int i = 0; i < 2; ++i) { ptx::mbar_init(&p_full[i], 16); ptx::mbar_init(&p_empty[i], 1); }
     ptx::mbar_init(o_free, 16);
     *abort_flag = misaligned ? 1 : 0;
     ptx::mbar_fence_init();
@@ -514,10 +515,11 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       look_up();
 #pragma unroll 1
       for (int u = warp == 1 ? 0 : 1; u < 4; u += 2) {
-        ok = ptx::mbar_spin_warp(&v_empty[u], (n & 1) ^ 1, abort_flag);
+        const uint32_t v = n * 4 + u, use = v / kSpaVUnits, slot = v - use * kSpaVUnits;
+        ok = ptx::mbar_spin_warp(&v_empty[slot], (use & 1) ^ 1, abort_flag);
         if (!ok) break;
-        const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaVUnit;
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[u], 2 * kSpaVUnit);
+        const uint32_t bar = bar0 + slot * 8, dst = dst0 + slot * kSpaVUnit;
+        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[slot], 2 * kSpaVUnit);
         if ((wide >> (u * 8)) & 1) {
           const int32_t y = __shfl_sync(0xffffffffu, r[0], u * 8);
           if (lane == 0) ptx::tma_load_5d_pair(dst, &tmap_v32, bar, 0, y, 0, 0, (int32_t)rank);
@@ -616,23 +618,25 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         ok = ptx::mbar_spin_cluster_warp(o_free, (n_job & 1) ^ 1, abort_flag);
         const int32_t first = w.tile(), stop = w.stop();
         for (int32_t t = first; t < stop && ok; ++t, ++n) {
-          ok = ptx::mbar_spin_cluster_warp(p_full, n & 1, abort_flag);
+          ok = ptx::mbar_spin_cluster_warp(&p_full[n & 1], (n >> 1) & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int u = 0; u < 4; ++u) {
-            ok = ptx::mbar_spin_warp(&v_full[u], n & 1, abort_flag);
+            const uint32_t v = n * 4 + u, use = v / kSpaVUnits, slot = v - use * kSpaVUnits;
+            ok = ptx::mbar_spin_warp(&v_full[slot], use & 1, abort_flag);
             if (!ok) break;
             if (ptx::elect_one()) {
-              const uint32_t pl = (uint32_t)pd + (u >> 1) * (kSpaPBlk / 16) + (u & 1) * 4, vl = (uint32_t)vd + u * (kSpaVUnit / 16);
+              const uint32_t pl = (uint32_t)pd + (n & 1) * (kSpaPBuf / 16) + (u >> 1) * (kSpaPBlk / 16) + (u & 1) * 4;
+              const uint32_t vl = (uint32_t)vd + slot * (kSpaVUnit / 16);
 #pragma unroll
               for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
                   ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (8192 / 16) + kk * (2048 / 16), v_hi,
                                       a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
-              ptx::mma_commit_pair(&v_empty[u]);
-              if (u == 3) ptx::mma_commit_pair(p_empty);
+              ptx::mma_commit_pair(&v_empty[slot]);
+              if (u == 3) ptx::mma_commit_pair(&p_empty[n & 1]);
             }
             __syncwarp();
           }
@@ -648,7 +652,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const int trow = (int)rank * 64 + hl;         // row of the tile
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_empty_lead0 = ptx::map_to_rank(&s_empty[0], 0), s_empty_lead1 = ptx::map_to_rank(&s_empty[1], 0);
-    const uint32_t p_full_lead = ptx::map_to_rank(p_full, 0), o_free_lead = ptx::map_to_rank(o_free, 0);
+    const uint32_t p_full_lead = ptx::map_to_rank(&p_full[0], 0), o_free_lead = ptx::map_to_rank(o_free, 0);
     uint64_t* xb = &x_bar[quarter & 1];
     uint32_t n = 0, n_x = 0;
     bool ok = true;
@@ -740,7 +744,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           l *= f;
           m_ref = m_new;
           if (t > first) {
-            ok = ptx::mbar_spin_warp(p_empty, (n - 1) & 1, abort_flag);     // O is complete up to the tile before
+            ok = ptx::mbar_spin_warp(&p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag);     // O is complete up to the tile before
             if (!ok) break;
             ptx::tc_fence_after();
 #pragma unroll 1
@@ -767,11 +771,11 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           pw[k / 2 + 1] = pack2(e2, e3, a.is_bf16);
         }
         l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
-        // P once the value products of the tile before have read theirs
-        ok = ptx::mbar_spin_warp(p_empty, (n & 1) ^ 1, abort_flag);
+        // P once the value products of the tile before the last have read theirs
+        ok = ptx::mbar_spin_warp(&p_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
         if (!ok) break;
         {
-          unsigned char* prow = p_s + half * kSpaPBlk + hl * 128;   // keys half * 64 .. are the first or second 64
+          unsigned char* prow = p_s + b * kSpaPBuf + half * kSpaPBlk + hl * 128;   // keys half * 64 .. are the first or second 64
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4*>(prow + (((g * 4 + c) ^ (hl & 7)) << 4)) =
@@ -779,7 +783,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
-        signal_lead(p_full, p_full_lead, true);
+        signal_lead(&p_full[b], p_full_lead + b * 8, true);
       }
       if (!ok) break;
       // ---- the row's sum, then O
@@ -791,7 +795,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         const int32_t tok = (j.row0 + trow) / a.p.n1;
         if (trow < j.nrows && !j.packed && atomicExch(&a.p.redo[tok], 1) == 0) a.p.redo_list[atomicAdd(a.p.redo_count, 1)] = tok;
       }
-      ok = ptx::mbar_spin_warp(p_empty, (n - 1) & 1, abort_flag);
+      ok = ptx::mbar_spin_warp(&p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
       const bool any = l_row != 0.f;                 // (a sum that is not a number stays one)
