@@ -253,11 +253,12 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int32_t x, int32_t y,
-                                                 int32_t z) {
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int32_t x, int32_t y,
+                                                 int32_t z, int32_t u) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u)
       : "memory");
 }
 __device__ __forceinline__ void tma_load_5d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar, int32_t x, int32_t y,
@@ -305,11 +306,12 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
 // Shared-memory matrix descriptor, K-major operand, 128-byte swizzle: rows of 128 bytes, groups
 // of 8 rows 1024 bytes apart.  `addr` must point into a 1024-byte aligned tile (it may be
 // advanced by 32-byte steps inside the swizzle atom to walk the K dimension).
-__device__ __forceinline__ uint64_t desc_kmajor_sw128(uint32_t addr) {
+// `sbo`: bytes between the groups of 8 rows, for tiles that hold something else in between.
+__device__ __forceinline__ uint64_t desc_kmajor_sw128(uint32_t addr, uint32_t sbo = 1024) {
   uint64_t d = 0;
   d |= (uint64_t)((addr & 0x3FFFFu) >> 4);        // start address
   d |= (uint64_t)1 << 16;                         // leading byte offset (unused for swizzled K-major)
-  d |= (uint64_t)(1024 >> 4) << 32;               // stride byte offset: 8 rows * 128 B
+  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;    // stride byte offset: 8 rows * 128 B where they are dense
   d |= (uint64_t)1 << 46;                         // descriptor version (Blackwell)
   d |= (uint64_t)2 << 61;                         // SWIZZLE_128B
   return d;

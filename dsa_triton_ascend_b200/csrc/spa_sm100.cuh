@@ -22,8 +22,8 @@
 // O 256 columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off, so that a score is too small by
 // 5e-7 of itself after 36 steps, and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
 //
-// Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, 16 of them per box where the page size is a
-// multiple of 16, else (and at the ends of a range, where some of 16 are not wanted) with gather4, four rows each; rows
+// Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, as many per box (64, 32, 16, 8) as divide the
+// page size, else (and at the ends of a range, where some of 8 are not wanted) with gather4, four rows each; rows
 // that are not wanted and absent pages are read at a row past the tensor, which gives zeros without touching
 // memory: what lies behind a sequence's end never enters a product.  Bytes are counted on the even CTA's barriers, where
 // the products are issued.  Rings: K five units of 64 keys x 128 features (the fifth, the rope, 64), one tile,
@@ -57,12 +57,19 @@ constexpr int kSpaQkWarp0 = 3, kSpaSoftWarp0 = 4, kSpaPvWarp = 12, kSpaQkWarp1 =
 constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
 constexpr int kSpaPackKeys = 256;    // a shorter prefix is not worth the partials
 constexpr int kSpaPlanThreads = 1024;
+constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
+constexpr int kSpaSnapTiles = 3;     // tiles that a share may be longer by so that it ends with its job
 
 constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
 constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
 constexpr uint32_t kSpaBlk = 64 * 128;                      // 64 keys x 64 features
-constexpr uint32_t kSpaKUnit = 2 * kSpaBlk;                 // two such blocks; the fifth unit, the rope, is one
-constexpr uint32_t kSpaVUnit = 4 * 32 * 128;                // 32 keys x four blocks of 64 columns
+// Pages of 64 (or multiples): a unit is one box, block after block (K [2 blocks][64 keys][128 bytes], V [4 blocks of columns]
+// [32 keys][128 bytes]).  Other pages: groups of 8 keys (1024 bytes per 64 features, one swizzle atom), all of a group's
+// blocks together, so that a box of 32, 16 or 8 keys is in one piece: K [8 groups][2 blocks][8 keys], V [4 groups][4
+// blocks][8 keys].  The second order costs 1-3 % (attend 64 x 128 heads, pages of 128: 246 -> 253 us), one load per
+// block and 16 keys in the first 25 % (pages of 16: 105 -> 86 us).
+constexpr uint32_t kSpaKUnit = 2 * kSpaBlk;                 // 64 keys x 128 features; the fifth unit, the rope, has 64
+constexpr uint32_t kSpaVUnit = 4 * 32 * 128;                // 32 keys x 256 columns
 constexpr uint32_t kSpaPBlk = 64 * 128;                     // 64 rows x 64 keys
 constexpr uint32_t kSpaPBuf = 2 * kSpaPBlk;
 constexpr uint32_t kSpaVUnits = 3;                          // units in the ring (a tile has four)
@@ -91,9 +98,15 @@ struct SpaJob {
 static_assert(sizeof(SpaJob) == 48, "three 16-byte loads");
 
 struct SpaPlan {
-  int32_t jobs, tiles, share;   // share: tiles per CTA pair
-  int32_t prefix, ref;          // positions shared, and the sequence whose pages they are read from
+  int32_t share;                // tiles per CTA pair
+  int32_t prefix;               // positions shared
 };
+// A CTA pair's share: tiles at .. end - 1, from job `index` on.
+struct SpaStart {
+  int32_t at, end, index, unused;
+  SpaJob j;
+};
+static_assert(sizeof(SpaStart) == 64, "four 16-byte loads");
 
 struct SpaDev {
   SeqDesc seq;              // seq_k: keys with the prefix; paged
@@ -106,8 +119,8 @@ struct SpaDev {
   // workspace
   SpaPlan* plan;
   SpaJob* job;              // [prefix_tiles + own_tiles]
-  int32_t* job_of;          // [prefix_tiles + own_tiles] job of a row tile, -1: none
-  int32_t* first_job;       // [clusters] job of a pair's first tile
+  int2* place;              // [prefix_tiles + own_tiles] job of a row tile (-1: none), and its sequence
+  SpaStart* start;          // [clusters]
   int32_t* redo;            // [rows]
   int32_t* redo_list;       // [rows]
   int32_t* redo_count;
@@ -122,7 +135,7 @@ struct SpaDev {
   int32_t return_lse;
 };
 
-// What the plan and the kernels that follow it agree on about a sequence.
+// What the plan and the kernels that follow it agree on about a sequence (b = batch: the rows behind the last one).
 struct SpaSeq {
   int32_t start, act_q, act_k;   // first token, query tokens (within the tensor), keys (within the table)
   int32_t vis0;                  // positions that its first token sees (may be negative)
@@ -131,6 +144,12 @@ struct SpaSeq {
 __device__ __forceinline__ SpaSeq spa_seq(const SpaDev& p, int32_t b, int32_t prefix) {
   SpaSeq s;
   int32_t act_q;
+  if (b >= p.seq.batch) {            // the rows behind the last sequence (TND)
+    s.start = min(max(p.seq.seq_q[p.seq.batch - 1], 0), p.rows);
+    s.act_q = s.act_k = s.vis0 = 0;
+    s.packed = false;
+    return s;
+  }
   if (p.seq.layout_q == DSA_LAYOUT_TND) {
     s.start = b > 0 ? p.seq.seq_q[b - 1] : 0;
     act_q = p.seq.seq_q[b] - s.start;
@@ -160,6 +179,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
   __shared__ unsigned long long best_s[32];
   __shared__ int32_t sum_s[3][33];
   __shared__ int32_t total_s[3];
+  __shared__ int32_t tiles_s[kSpaClusters];   // tiles of the first jobs
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dep_launch();
   grid_dep_wait();
@@ -192,6 +212,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     SpaJob j;
     j.tiles = 0;
     j.slot = -1;
+    int32_t of_seq = 0;
     if (f < p.prefix_tiles) {
       j.row0 = f * kSpaRows;
       j.nrows = min(kSpaRows, rows - j.row0);
@@ -219,13 +240,14 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
       int32_t b;
       if (p.seq.layout_q != DSA_LAYOUT_TND) b = g / p.own_tiles_per_seq;
       else {
-        int32_t lo = 0, hi = p.seq.batch - 1;      // the last sequence whose first place is g or before
+        int32_t lo = 0, hi = p.seq.batch;      // the last sequence (or the rows behind them) whose first place is g or before
         while (lo < hi) {
           const int32_t mid = (lo + hi + 1) >> 1;
           if (spa_own_place(p, mid, min(max(p.seq.seq_q[mid - 1], 0), p.rows)) <= g) lo = mid; else hi = mid - 1;
         }
         b = lo;
       }
+      of_seq = b;
       const SpaSeq s = spa_seq(p, b, prefix);
       const int32_t i = g - spa_own_place(p, b, s.start), n = s.act_q * p.n1;
       j.row0 = s.start * p.n1 + i * kSpaRows;
@@ -271,25 +293,71 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     __syncthreads();
     if (f < places) {
       const int32_t at = jobs + sum_s[0][warp] + x[0] - v[0];
-      p.job_of[f] = v[0] ? at : -1;
+      p.place[f] = make_int2(v[0] ? at : -1, of_seq);
       if (v[0]) {
         j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1];
         if (v[2]) j.slot = 2 * p.clusters + packed + sum_s[2][warp] + x[2] - v[2];
         p.job[at] = j;
+        if (at < kSpaClusters) tiles_s[at] = j.tiles;
       }
     }
     jobs += total_s[0]; tiles += total_s[1]; packed += total_s[2];
     __syncthreads();
   }
-  const int32_t share = max(1, (tiles + p.clusters - 1) / p.clusters);
-  if (tid == 0) {
-    SpaPlan w;
-    w.jobs = jobs; w.tiles = tiles; w.share = share; w.prefix = prefix; w.ref = ref;
-    *p.plan = w;
+  int32_t share = max(1, (tiles + p.clusters - 1) / p.clusters);
+  // Few jobs: shares that end with their jobs save a pair its second job (a load of Q, a partial) for tiles that its neighbours
+  // do not have.  Warp w tries shares longer by w tiles; the first that needs no more than one share per pair is
+  // taken: the places of the jobs' tiles are then rounded up to whole shares.
+  bool single = false;
+  if (jobs > 0 && jobs <= kSpaClusters) {
+    const int32_t try_share = share + warp;
+    int32_t parts = 0;
+    for (int32_t i = lane; i < jobs; i += 32) parts += (tiles_s[i] + try_share - 1) / try_share;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) parts += __shfl_xor_sync(0xffffffffu, parts, o);
+    if (lane == 0) sum_s[0][warp] = parts;
+    __syncthreads();
+    int32_t extra = 0;
+    while (extra <= kSpaSnapTiles && sum_s[0][extra] > p.clusters) ++extra;
+    if (extra <= kSpaSnapTiles) {
+      single = true;
+      share += extra;
+      if (warp == 0) {
+        int32_t before = 0;
+        for (int32_t i0 = 0; i0 < jobs; i0 += 32) {
+          const int32_t i = i0 + lane, mine = i < jobs ? (tiles_s[i] + share - 1) / share : 0;
+          int32_t z = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int32_t y = __shfl_up_sync(0xffffffffu, z, o);
+            if (lane >= o) z += y;
+          }
+          if (i < jobs) p.job[i].tile0 = (before + z - mine) * share;
+          before += __shfl_sync(0xffffffffu, z, 31);
+        }
+        if (lane == 0) total_s[1] = before * share;
+      }
+      __syncthreads();
+      tiles = total_s[1];
+    }
   }
+  if (tid == 0) {
+    p.plan->share = share;
+    p.plan->prefix = prefix;
+  }
+  for (int32_t c = tid; c < p.clusters; c += kSpaPlanThreads)
+    if ((int64_t)c * share >= tiles) p.start[c].at = p.start[c].end = 0;
   for (int32_t i = tid; i < jobs; i += kSpaPlanThreads) {
-    const int32_t t0 = p.job[i].tile0, t1 = t0 + p.job[i].tiles;
-    for (int32_t c = (t0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) p.first_job[c] = i;
+    SpaStart w;
+    w.j = p.job[i];
+    w.index = i;
+    w.unused = 0;
+    const int32_t t1 = w.j.tile0 + w.j.tiles;
+    for (int32_t c = (w.j.tile0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
+      w.at = c * share;
+      w.end = min(w.at + share, single ? t1 : tiles);
+      p.start[c] = w;
+    }
   }
 }
 
@@ -310,15 +378,15 @@ __device__ __forceinline__ SpaJob spa_load_job(const SpaJob* p) {
 // Walks over the tiles of a pair's share.
 struct SpaWalk {
   const SpaJob* jobs;
-  int32_t at, end, index;    // tile in the order of all tiles, end of the share, job
+  int32_t at, end, index;
   SpaJob j;
   __device__ __forceinline__ void start(const SpaDev& p, int32_t cluster) {
-    const SpaPlan w = *p.plan;
     jobs = p.job;
-    at = min((int64_t)cluster * w.share, (int64_t)w.tiles);
-    end = min(at + w.share, w.tiles);
-    index = 0;
-    if (at < end) { index = p.first_job[cluster]; j = spa_load_job(jobs + index); }
+    SpaStart w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&w)[i] = reinterpret_cast<const int4*>(p.start + cluster)[i];
+    at = w.at; end = w.end; index = w.index;
+    j = w.j;
   }
   __device__ __forceinline__ bool more() const { return at < end; }
   __device__ __forceinline__ int32_t tile() const { return at - j.tile0; }                       // of the job
@@ -337,6 +405,8 @@ struct SpaArgs {
   uint32_t idesc_qk, idesc_pv;
   float scale_log2;
   int32_t is_bf16, key_rows, blocks;
+  int32_t box_keys;                // 64, 32, 16 or 8: keys per box
+  int32_t k_group, k_block, v_group, v_block;   // bytes from a group of 8 keys, and from a block of 64 columns, to the next
   uint32_t page_mul, page_shift;   // position / page size = position * page_mul >> page_shift (positions below 2^31)
 };
 
@@ -367,10 +437,10 @@ __device__ __forceinline__ bool spa_box(const SpaArgs& a, const SpaJob& j, int32
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSpaThreads, 1)
 spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_qr,
-                     const __grid_constant__ CUtensorMap tmap_k64, const __grid_constant__ CUtensorMap tmap_r64,
-                     const __grid_constant__ CUtensorMap tmap_k16, const __grid_constant__ CUtensorMap tmap_r16,
+                     const __grid_constant__ CUtensorMap tmap_kh, const __grid_constant__ CUtensorMap tmap_rh,
+                     const __grid_constant__ CUtensorMap tmap_k8, const __grid_constant__ CUtensorMap tmap_r8,
                      const __grid_constant__ CUtensorMap tmap_k1, const __grid_constant__ CUtensorMap tmap_r1,
-                     const __grid_constant__ CUtensorMap tmap_v32, const SpaArgs a) {
+                     const __grid_constant__ CUtensorMap tmap_vh, const SpaArgs a) {
   extern __shared__ __align__(1024) unsigned char spa_sm[];
   unsigned char* q_s = spa_sm + kSpaOffQ;
   unsigned char* k_s = spa_sm + kSpaOffK;
@@ -429,21 +499,25 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     // nothing started
   } else if (warp == 0 || warp == kSpaKWarp1) {
     // ------------------------------------------------------------------ K loads
-    // Two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3.  Lane 4 g + i of the first 16 holds positions
-    // 16 g + 4 i .. + 3 of this CTA's 64.  A unit is one box where the 64 lie in one page, else a box or four gathers per
-    // 16 keys and 64 features.  One lane issues: lanes that each issue their own cost 130 cycles a load.
+    // Two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3.  Lane 2 g + i of the first 16 holds positions
+    // 8 g + 4 i .. + 3 of this CTA's 64.  Boxes are as high as pages allow (64, 32, 16 or 8 keys); where a box would
+    // reach past the wanted positions it is cut into groups of 8, and a group that is cut itself (or every one, where pages
+    // are no multiple of 8) is gathered, four rows a time.  One lane issues: lanes that each issue their own cost 130
+    // cycles a load.
     const uint32_t dst0 = ptx::smem_u32(k_s), bar0 = ptx::map_to_rank(&k_full[0], 0);
     const int u0 = warp == 0 ? 0 : 2, units = warp == 0 ? 3 : 2;
+    const int high = a.box_keys / 8;                   // groups per box
+    const bool dense = a.box_keys == 64;
     SpaWalk w;
     w.start(a.p, cluster);
     SpaQuad quad;
-    bool box64 = false, box16 = false;
+    bool box = false, box8 = false;
     auto look_up = [&]() {
       if (!w.more()) return;
-      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64;
-      box64 = spa_box(a, w.j, pos, 64);
-      box16 = spa_box(a, w.j, pos + (lane & ~3) * 4, 16);
-      quad.look_up(a, w.j, pos + (lane & 15) * 4);
+      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64 + (lane & 15) * 4;
+      box = spa_box(a, w.j, pos & -a.box_keys, a.box_keys);
+      box8 = spa_box(a, w.j, pos & ~7, 8);
+      quad.look_up(a, w.j, pos);
     };
     look_up();
     bool ok = true;
@@ -451,8 +525,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int32_t r[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
-      const bool one = box64;
-      const uint32_t boxes = __ballot_sync(0xffffffffu, box16);
+      const uint32_t boxes = __ballot_sync(0xffffffffu, box), boxes8 = __ballot_sync(0xffffffffu, box8);
       w.next_tile();
       look_up();
 #pragma unroll 1
@@ -462,47 +535,68 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaKUnit;
         if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[u], u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
-        if (one) {
-          if (lane == 0) {
-            if (u < 4) ptx::tma_load_3d_pair(dst, &tmap_k64, bar, 0, r[0], u * 2);
-            else ptx::tma_load_2d_pair(dst, &tmap_r64, bar, 0, r[0]);
-          }
-        } else {
 #pragma unroll 1
-          for (int q = 0; q < 16; ++q) {
-            const int32_t y0 = __shfl_sync(0xffffffffu, r[0], q), y1 = __shfl_sync(0xffffffffu, r[1], q),
-                          y2 = __shfl_sync(0xffffffffu, r[2], q), y3 = __shfl_sync(0xffffffffu, r[3], q);
-            const bool box = (boxes >> q) & 1;
+        for (int g = 0; g < 8;) {
+          const int32_t y0 = __shfl_sync(0xffffffffu, r[0], 2 * g);
+          const bool tall = (boxes >> (2 * g)) & 1;
+          if (tall) {
             if (lane == 0) {
-#pragma unroll 1
-              for (int e = 0; e < (u < 4 ? 2 : 1); ++e) {
-                const uint32_t at = dst + e * kSpaBlk + q * 512;
-                const int32_t x = u < 4 ? u * 128 + e * 64 : 0;
-                if (box) ptx::tma_load_2d_pair(at, u < 4 ? &tmap_k16 : &tmap_r16, bar, x, y0);
-                else ptx::tma_gather4_2d_pair(at, u < 4 ? &tmap_k1 : &tmap_r1, bar, x, y0, y1, y2, y3);
+              if (u < 4) ptx::tma_load_4d_pair(dst + g * a.k_group, &tmap_kh, bar, u * 128, dense ? y0 : 0, 0, dense ? 0 : (y0 + 7) >> 3);
+              else ptx::tma_load_2d_pair(dst + g * 1024, &tmap_rh, bar, 0, y0);
+            }
+            g += high;
+            continue;
+          }
+          if ((boxes8 >> (2 * g)) & 1) {
+            if (lane == 0) {
+              if (u < 4) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  ptx::tma_load_2d_pair(dst + g * a.k_group + e * a.k_block, &tmap_k8, bar, u * 128 + e * 64, y0);
+              } else {
+                ptx::tma_load_2d_pair(dst + g * 1024, &tmap_r8, bar, 0, y0);
               }
             }
-            if (box) q += 3;
+            ++g;
+            continue;
           }
+#pragma unroll 1
+          for (int q = 2 * g; q < 2 * g + 2; ++q) {
+            const int32_t x0 = __shfl_sync(0xffffffffu, r[0], q), x1 = __shfl_sync(0xffffffffu, r[1], q),
+                          x2 = __shfl_sync(0xffffffffu, r[2], q), x3 = __shfl_sync(0xffffffffu, r[3], q);
+            if (lane == 0) {
+              if (u < 4) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  ptx::tma_gather4_2d_pair(dst + g * a.k_group + e * a.k_block + (q & 1) * 512, &tmap_k1, bar, u * 128 + e * 64, x0, x1, x2, x3);
+              } else {
+                ptx::tma_gather4_2d_pair(dst + q * 512, &tmap_r1, bar, 0, x0, x1, x2, x3);
+              }
+            }
+          }
+          ++g;
         }
         __syncwarp();
       }
     }
   } else if (warp == 1 || warp == kSpaVWarp1) {
     // ------------------------------------------------------------------ V loads
-    // Two warps, 1 has the units (32 keys x 256 columns) 0 and 2, 15 the units 1 and 3.  Lane 4 g + i holds positions
-    // 16 g + 4 i .. + 3 of the tile's 128.  A unit is one box, or a box or four gathers per 16 keys and 64 columns.
+    // Two warps, 1 has the units (32 keys x 256 columns) 0 and 2, 15 the units 1 and 3.  Lane 2 g + i holds positions
+    // 8 g + 4 i .. + 3 of the tile's 128; boxes as for K, of up to 32 keys.
     const uint32_t dst0 = ptx::smem_u32(v_s), bar0 = ptx::map_to_rank(&v_full[0], 0);
+    const int32_t box_keys = min(a.box_keys, 32);
+    const int high = box_keys / 8;
+    const bool dense = a.box_keys == 64;
     SpaWalk w;
     w.start(a.p, cluster);
     SpaQuad quad;
-    bool box32 = false, box16 = false;
+    bool box = false, box8 = false;
     auto look_up = [&]() {
       if (!w.more()) return;
-      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys;
-      box32 = spa_box(a, w.j, pos + (lane & ~7) * 4, 32);
-      box16 = spa_box(a, w.j, pos + (lane & ~3) * 4, 16);
-      quad.look_up(a, w.j, pos + lane * 4);
+      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + lane * 4;
+      box = spa_box(a, w.j, pos & -box_keys, box_keys);
+      box8 = spa_box(a, w.j, pos & ~7, 8);
+      quad.look_up(a, w.j, pos);
     };
     look_up();
     bool ok = true;
@@ -510,7 +604,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int32_t r[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
-      const uint32_t wide = __ballot_sync(0xffffffffu, box32), boxes = __ballot_sync(0xffffffffu, box16);
+      const uint32_t boxes = __ballot_sync(0xffffffffu, box), boxes8 = __ballot_sync(0xffffffffu, box8);
       w.next_tile();
       look_up();
 #pragma unroll 1
@@ -520,27 +614,40 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         const uint32_t bar = bar0 + slot * 8, dst = dst0 + slot * kSpaVUnit;
         if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[slot], 2 * kSpaVUnit);
-        if ((wide >> (u * 8)) & 1) {
-          const int32_t y = __shfl_sync(0xffffffffu, r[0], u * 8);
-          if (lane == 0) ptx::tma_load_5d_pair(dst, &tmap_v32, bar, 0, y, 0, 0, (int32_t)rank);
-        } else {
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            const int q = u * 8 + i;
-            const int32_t y0 = __shfl_sync(0xffffffffu, r[0], q), y1 = __shfl_sync(0xffffffffu, r[1], q),
-                          y2 = __shfl_sync(0xffffffffu, r[2], q), y3 = __shfl_sync(0xffffffffu, r[3], q);
-            const bool box = (boxes >> q) & 1;
-            if (lane == 0) {
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                const uint32_t at = dst + c * 4096 + i * 512;
-                const int32_t x = (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64;
-                if (box) ptx::tma_load_2d_pair(at, &tmap_k16, bar, x, y0);
-                else ptx::tma_gather4_2d_pair(at, &tmap_k1, bar, x, y0, y1, y2, y3);
-              }
-            }
-            if (box) i += 3;
+        for (int g = 0; g < 4;) {
+          const int l = (u * 4 + g) * 2;
+          const int32_t y0 = __shfl_sync(0xffffffffu, r[0], l);
+          const bool tall = (boxes >> l) & 1;
+          if (tall) {
+            if (lane == 0)
+              ptx::tma_load_5d_pair(dst + g * a.v_group, &tmap_vh, bar, (int32_t)rank * 128, dense ? y0 : 0, 0, 0,
+                                    dense ? 0 : (y0 + 7) >> 3);
+            g += high;
+            continue;
           }
+          if ((boxes8 >> l) & 1) {
+            if (lane == 0) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                ptx::tma_load_2d_pair(dst + g * a.v_group + c * a.v_block, &tmap_k8, bar,
+                                      (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, y0);
+            }
+            ++g;
+            continue;
+          }
+#pragma unroll 1
+          for (int q = 0; q < 2; ++q) {
+            const int32_t x0 = __shfl_sync(0xffffffffu, r[0], l + q), x1 = __shfl_sync(0xffffffffu, r[1], l + q),
+                          x2 = __shfl_sync(0xffffffffu, r[2], l + q), x3 = __shfl_sync(0xffffffffu, r[3], l + q);
+            if (lane == 0) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                ptx::tma_gather4_2d_pair(dst + g * a.v_group + c * a.v_block + q * 512, &tmap_k1, bar,
+                                         (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
+            }
+          }
+          ++g;
         }
         __syncwarp();
       }
@@ -571,8 +678,9 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
-      const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
-      const uint32_t q_hi = (uint32_t)(qd >> 32), k_hi = (uint32_t)(kd >> 32);
+      const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s), a.k_group);
+      const uint64_t rd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
+      const uint32_t q_hi = (uint32_t)(qd >> 32), k_block = a.k_block / 16;
       const uint32_t tm = tmem + kSpaTmS + (second ? 64 : 0);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
@@ -590,11 +698,12 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             if (!ok) break;
             if (ptx::elect_one()) {
               const uint32_t ql = (uint32_t)qd + u * (2 * kSpaQBlk / 16), kl = (uint32_t)kd + u * (kSpaKUnit / 16);
+              const uint32_t k_hi = (uint32_t)((u < 4 ? kd : rd) >> 32);
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)   // (addresses in a descriptor count 16 bytes)
                 if (kk < 4 || u < 4)
                   ptx::mma_ss_pair_lo(tm + b * 128, ql + (kk >> 2) * (kSpaQBlk / 16) + (kk & 3) * 2, q_hi,
-                                      kl + (kk >> 2) * (kSpaBlk / 16) + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
+                                      kl + (kk >> 2) * k_block + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
               ptx::mma_commit_pair(&k_empty[u]);
               if (i == units - 1) ptx::mma_commit_pair(&s_full[b]);
             }
@@ -611,8 +720,9 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
-      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 4096, 1024);
+      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), a.v_block, a.v_group);
       const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
+      const uint32_t v_half = 2 * a.v_block / 16, v_step = 2 * a.v_group / 16;   // two blocks of columns, 16 keys
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
         ok = ptx::mbar_spin_cluster_warp(o_free, (n_job & 1) ^ 1, abort_flag);
@@ -633,7 +743,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (8192 / 16) + kk * (2048 / 16), v_hi,
+                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * v_half + kk * v_step, v_hi,
                                       a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
               ptx::mma_commit_pair(&v_empty[slot]);
               if (u == 3) ptx::mma_commit_pair(&p_empty[n & 1]);
@@ -863,92 +973,126 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   if (threadIdx.x == 0 && *abort_flag) atomicExch(a.p.status, misaligned ? 2 : 1);
 }
 
-// ---- join: a warp per (token, head) whose result is in parts, or that sees nothing ------------------
-constexpr int kSpaJoinWarps = 8;
-__global__ void __launch_bounds__(kSpaJoinWarps * 32) spa_join_kernel(const SpaDev p, int32_t is_bf16) {
+// ---- join: the rows whose result is in parts, or that see nothing ----------------------------------
+// A block takes some rows of a row tile: where their parts are is the same for all of them (but for the prefix tile of a packed
+// sequence, one of two), and a tile that its job has written itself is left at once.  kWarps warps join a row, with 2 kWarps
+// parts' loads in flight: one where there are rows enough, four where there are few (8 x 16 heads behind 8192 tokens,
+// where a row has 60 parts: 44 -> 33 us a call; 64 x 128 heads, two parts: 25 us with four, 15 with one).
+constexpr int kSpaJoinThreads = 256;
+struct SpaParts { int32_t first, count, uncut; };      // first share, number of shares, partial of a job in one share
+__device__ __forceinline__ SpaParts spa_parts(const SpaDev& p, int32_t job, int32_t share) {
+  SpaParts w = {0, 0, -1};
+  if (job >= 0) {
+    const int32_t t0 = p.job[job].tile0, n = p.job[job].tiles;
+    w.uncut = p.job[job].slot;
+    w.first = t0 / share;
+    w.count = (t0 + n - 1) / share - w.first + 1;
+  }
+  return w;
+}
+template <int kWarps>
+__global__ void __launch_bounds__(kSpaJoinThreads, kWarps == 1 ? 3 : 2) spa_join_kernel(const SpaDev p, int32_t rows_per_block, int32_t is_bf16) {
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31;
-  const int32_t tok = blockIdx.x, h = blockIdx.y * kSpaJoinWarps + (threadIdx.x >> 5);
-  if (h >= p.n1) return;
-  const SpaPlan w = *p.plan;
-  const RowInfo ri = row_info(p.seq, tok);
-  const SpaSeq s = spa_seq(p, ri.b, w.prefix);
-  const int64_t row = (int64_t)tok * p.n1 + h;
-  // parts of the row: tiles of its own job, then of the prefix job
-  int32_t first[2] = {0, 0}, count[2] = {0, 0}, uncut[2] = {-1, -1}, trow[2] = {0, 0};
-  if (tok - s.start < s.act_q) {
-    const int32_t r = (tok - s.start) * p.n1 + h;
-    int32_t place[2] = {p.prefix_tiles + spa_own_place(p, ri.b, s.start) + r / kSpaRows, (int32_t)(row / kSpaRows)};
-    trow[0] = r % kSpaRows;
-    trow[1] = (int32_t)(row % kSpaRows);
+  const int32_t share = p.plan->share, prefix = p.plan->prefix;
+  const int2 mine = p.place[p.prefix_tiles + blockIdx.x];
+  const SpaSeq s = spa_seq(p, mine.y, prefix);
+  const int32_t i = (int32_t)blockIdx.x - spa_own_place(p, mine.y, s.start);
+  const int32_t tokens = p.seq.layout_q != DSA_LAYOUT_TND ? p.seq.s1 : (mine.y < p.seq.batch ? s.act_q : p.rows - s.start);
+  if (i < 0) return;
+  const int32_t row0 = s.start * p.n1 + i * kSpaRows;
+  const int32_t total = min(kSpaRows, tokens * p.n1 - i * kSpaRows), active = min(total, s.act_q * p.n1 - i * kSpaRows);
+  const SpaParts own = spa_parts(p, mine.x, share);
+  const bool written = own.count == 1 && own.uncut < 0;      // the job wrote its rows itself
+  const int32_t r0 = (int32_t)blockIdx.y * rows_per_block, r1 = min(r0 + rows_per_block, total);
+  if (r0 >= total || (written && r1 <= active)) return;
+  SpaParts pre[2] = {{0, 0, -1}, {0, 0, -1}};
+  const int32_t pre0 = row0 / kSpaRows;
+  if (s.packed) {
+    pre[0] = spa_parts(p, p.place[pre0].x, share);
+    if ((row0 + total - 1) / kSpaRows > pre0) pre[1] = spa_parts(p, p.place[pre0 + 1].x, share);
+  }
+  constexpr int kCols = 4 / kWarps, kFly = 2 * kWarps;             // groups of four columns per lane; parts in flight
+  const int col = (int)((threadIdx.x >> 5) % kWarps) * 32 + lane;
+  for (int32_t r = r0 + (threadIdx.x >> 5) / kWarps; r < r1; r += kSpaJoinThreads / 32 / kWarps) {
+    if (written && r < active) continue;
+    const int64_t row = row0 + r;
+    const bool second = row / kSpaRows > pre0;
+    const int32_t p_first = second ? pre[1].first : pre[0].first, p_uncut = second ? pre[1].uncut : pre[0].uncut;
+    const int32_t p_count = r < active ? (second ? pre[1].count : pre[0].count) : 0;
+    const int32_t o_count = r < active ? own.count : 0, parts = o_count + p_count;
+    // partial of part k: a job's first share leaves it at 2 c + 1, the later ones at 2 c
+    auto at = [&](int32_t k) -> int64_t {
+      const bool o = k < o_count;
+      if (!o) k -= o_count;
+      const int32_t m = o ? o_count : p_count, c0 = o ? own.first : p_first;
+      const int32_t slot = m == 1 ? (o ? own.uncut : p_uncut) : 2 * (c0 + k) + (k == 0 ? 1 : 0);
+      return (int64_t)slot * kSpaRows + (o ? r : (int32_t)(row % kSpaRows));
+    };
+    // the first 32 parts' maxima and sums stay in the lanes
+    float m0 = 0.f, l0 = 0.f, mx = -INFINITY;
+    if (lane < parts) {
+      m0 = p.part_m[at(lane)];
+      l0 = p.part_l[at(lane)];
+      if (l0 != 0.f) mx = m0;
+    }
+    for (int32_t k = lane + 32; k < parts; k += 32)
+      if (p.part_l[at(k)] != 0.f) mx = fmaxf(mx, p.part_m[at(k)]);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (k == 1 && !s.packed) continue;
-      const int32_t i = p.job_of[place[k]];
-      if (i < 0) continue;
-      const int32_t t0 = p.job[i].tile0, t1 = t0 + p.job[i].tiles - 1;
-      first[k] = t0 / w.share;
-      count[k] = t1 / w.share - first[k] + 1;
-      if (count[k] == 1) {
-        uncut[k] = p.job[i].slot;
-        if (uncut[k] < 0) return;        // the job wrote the row itself
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float4 acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+    for (int32_t k0 = 0; k0 < parts; k0 += 32) {
+      float wt = 0.f;
+      if (k0 == 0) wt = l0 != 0.f ? l0 * ex2(m0 - mx) : 0.f;
+      else if (k0 + lane < parts) {
+        const float l = p.part_l[at(k0 + lane)];
+        if (l != 0.f) wt = l * ex2(p.part_m[at(k0 + lane)] - mx);
+      }
+      for (int32_t j0 = 0; j0 < 32 && k0 + j0 < parts; j0 += kFly) {
+        float f[kFly];
+        float4 v[kFly][kCols];
+#pragma unroll
+        for (int e = 0; e < kFly; ++e) {
+          f[e] = __shfl_sync(0xffffffffu, wt, j0 + e);
+          const float4* o = reinterpret_cast<const float4*>(p.part_o + at(k0 + j0 + e) * 512) + col;
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            v[e][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (f[e] != 0.f) v[e][c] = o[c * 32 * kWarps];      // (else O may never have been written)
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kFly; ++e) {
+          den += f[e];
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            acc[c].x += f[e] * v[e][c].x; acc[c].y += f[e] * v[e][c].y;
+            acc[c].z += f[e] * v[e][c].z; acc[c].w += f[e] * v[e][c].w;
+          }
+        }
       }
     }
-  }
-  const int32_t parts = count[0] + count[1];
-  // partial of part i: a job's first share leaves it at 2 c + 1, the later ones at 2 c
-  auto at = [&](int32_t i) -> int64_t {
-    const int k = i >= count[0];
-    if (k) i -= count[0];
-    const int32_t slot = count[k] == 1 ? uncut[k] : 2 * (first[k] + i) + (i == 0 ? 1 : 0);
-    return (int64_t)slot * kSpaRows + trow[k];
-  };
-  float mx = -INFINITY;
-  for (int32_t i = lane; i < parts; i += 32)
-    if (p.part_l[at(i)] != 0.f) mx = fmaxf(mx, p.part_m[at(i)]);
+    const bool any = den != 0.f;
+    const float inv = any ? 1.f / den : 0.f;
+    uint2* out = reinterpret_cast<uint2*>((unsigned char*)p.out + row * 1024) + col;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float4 acc[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.f;
-  for (int32_t i0 = 0; i0 < parts; i0 += 32) {
-    float wt = 0.f;
-    if (i0 + lane < parts) {
-      const float l = p.part_l[at(i0 + lane)];
-      if (l != 0.f) wt = l * ex2(p.part_m[at(i0 + lane)] - mx);
+    for (int c = 0; c < kCols; ++c)
+      out[c * 32 * kWarps] = make_uint2(pack2(acc[c].x * inv, acc[c].y * inv, is_bf16), pack2(acc[c].z * inv, acc[c].w * inv, is_bf16));
+    if (col == 0 && p.softmax_max != nullptr) {
+      const bool give = p.return_lse && any;
+      p.softmax_max[row] = give ? mx * 0.6931471805599453f : 0.f;
+      p.softmax_sum[row] = give ? den : 0.f;
     }
-    for (int32_t i = i0; i < min(parts, i0 + 32); ++i) {
-      const float f = __shfl_sync(0xffffffffu, wt, i - i0);
-      if (f == 0.f) continue;            // (its O may never have been written)
-      den += f;
-      const float4* o = reinterpret_cast<const float4*>(p.part_o + at(i) * 512);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 v = o[c * 32 + lane];
-        acc[c].x += f * v.x; acc[c].y += f * v.y; acc[c].z += f * v.z; acc[c].w += f * v.w;
-      }
-    }
-  }
-  const bool any = den != 0.f;
-  const float inv = any ? 1.f / den : 0.f;
-  uint2* out = reinterpret_cast<uint2*>((unsigned char*)p.out + row * 1024);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    out[c * 32 + lane] = make_uint2(pack2(acc[c].x * inv, acc[c].y * inv, is_bf16), pack2(acc[c].z * inv, acc[c].w * inv, is_bf16));
-  if (lane == 0 && p.softmax_max != nullptr) {
-    const bool give = p.return_lse && any;
-    p.softmax_max[row] = give ? mx * 0.6931471805599453f : 0.f;
-    p.softmax_sum[row] = give ? den : 0.f;
   }
 }
 
 // ---- host side ---------------------------------------------------------------------------------
-constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
-
 struct SpaWs {
-  size_t plan, job, job_of, first_job, redo, redo_list, redo_count, part_m, part_l, part_o, total;
+  size_t plan, job, place, start, redo, redo_list, redo_count, part_m, part_l, part_o, total;
   int64_t prefix_tiles, own_tiles, own_tiles_per_seq, slots;
   bool pack, redo_used;
 };
@@ -961,7 +1105,7 @@ inline SpaWs spa_ws_layout(const DsaSpaParams* p, int64_t rows) {
   w.pack = (p->prefix_device != nullptr || p->prefix >= kSpaPackKeys) && p->n1 <= kSpaPackRows;
   w.prefix_tiles = w.pack ? tiles(rows * p->n1) : 0;
   w.own_tiles_per_seq = tnd ? 0 : std::max<int64_t>(1, tiles((int64_t)p->s1 * p->n1));
-  w.own_tiles = tnd ? rows * p->n1 / kSpaRows + p->batch : p->batch * w.own_tiles_per_seq;
+  w.own_tiles = tnd ? rows * p->n1 / kSpaRows + p->batch + 1 : p->batch * w.own_tiles_per_seq;
   // a packed sequence has one tile of its own and touches two prefix tiles at most
   w.slots = 2 * kSpaClusters + (w.pack ? std::min<int64_t>(w.own_tiles, p->batch) + std::min<int64_t>(w.prefix_tiles, 2ll * p->batch) : 0);
   // rows of a tile see different keys only when it holds several tokens of a sequence under the causal mask
@@ -969,9 +1113,9 @@ inline SpaWs spa_ws_layout(const DsaSpaParams* p, int64_t rows) {
   const size_t places = (size_t)(w.prefix_tiles + w.own_tiles);
   w.plan = 0;
   w.job = 256;
-  w.job_of = w.job + up(places * sizeof(SpaJob));
-  w.first_job = w.job_of + up(places * 4);
-  w.redo_count = w.first_job + up(kSpaClusters * 4);
+  w.place = w.job + up(places * sizeof(SpaJob));
+  w.start = w.place + up(places * 8);
+  w.redo_count = w.start + up(kSpaClusters * sizeof(SpaStart));
   w.redo = w.redo_count + 256;
   w.redo_list = w.redo + (w.redo_used ? up((size_t)rows * 4) : 0);
   w.part_m = w.redo_list + (w.redo_used ? up((size_t)rows * 4) : 0);
@@ -1006,30 +1150,19 @@ inline bool spa_sm100_prepare(int dev) {
   return true;
 }
 
-// The latent cache [keys, 512] as [block 8][keys][64 features].  A box of 64 keys x two blocks is a K unit.
-inline bool spa_tmap_k(CUtensorMap* m, const void* base, uint64_t keys, bool bf16) {
+// The latent cache [keys, 512] as boxes of K units (64 features from 128 u on, both blocks) and of V units (64 columns from 128 c
+// on for CTA c, both blocks of both halves): `box_keys` rows, or as many of them in groups of 8.
+inline bool spa_tmap(CUtensorMap* m, const void* base, uint64_t keys, uint32_t box_keys, bool dense, bool v, bool bf16) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (enc == nullptr) return false;
-  cuuint64_t dims[3] = {64, keys, 8};
-  cuuint64_t strides[2] = {1024, 128};
-  cuuint32_t box[3] = {64, 64, 2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
-             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// The latent cache [keys, 512] as [rank 2][half 2][block 2][keys][64 columns]: column 256 half + 128 rank + 64 block.  A box of
-// 32 keys x both blocks x both halves is a V unit, 64-column blocks of 32 rows one behind the other.
-inline bool spa_tmap_v(CUtensorMap* m, const void* base, uint64_t keys, bool bf16) {
-  EncodeTiledFn enc = tensor_map_encoder();
-  if (enc == nullptr) return false;
-  cuuint64_t dims[5] = {64, keys, 2, 2, 2};
-  cuuint64_t strides[4] = {1024, 128, 512, 256};
-  cuuint32_t box[5] = {64, 32, 2, 2, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims,
-             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint64_t rows = dense ? keys : 8, groups = dense ? 1 : std::max<uint64_t>(keys / 8, 1);
+  const cuuint32_t r = dense ? box_keys : 8, g = dense ? 1 : box_keys / 8;
+  const cuuint64_t k_dims[4] = {512, rows, 2, groups}, k_strides[3] = {1024, 128, 8192};
+  const cuuint64_t v_dims[5] = {512, rows, 2, 2, groups}, v_strides[4] = {1024, 128, 512, 8192};
+  const cuuint32_t k_box[4] = {64, r, 2, g}, v_box[5] = {64, r, 2, 2, g}, estr[5] = {1, 1, 1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v ? 5 : 4, const_cast<void*>(base),
+             v ? v_dims : k_dims, v ? v_strides : k_strides, v ? v_box : k_box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // `dense`: the call for the row-by-row kernel.
@@ -1048,8 +1181,8 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   d.prefix_tiles = (int32_t)w.prefix_tiles; d.own_tiles = (int32_t)w.own_tiles; d.own_tiles_per_seq = (int32_t)w.own_tiles_per_seq;
   d.pack_rows = w.pack ? kSpaPackRows : 0;
   d.clusters = kSpaClusters;
-  d.plan = (SpaPlan*)(ws + w.plan); d.job = (SpaJob*)(ws + w.job); d.job_of = (int32_t*)(ws + w.job_of);
-  d.first_job = (int32_t*)(ws + w.first_job);
+  d.plan = (SpaPlan*)(ws + w.plan); d.job = (SpaJob*)(ws + w.job); d.place = (int2*)(ws + w.place);
+  d.start = (SpaStart*)(ws + w.start);
   d.redo = w.redo_used ? (int32_t*)(ws + w.redo) : nullptr;
   d.redo_list = (int32_t*)(ws + w.redo_list); d.redo_count = (int32_t*)(ws + w.redo_count);
   d.status = status;
@@ -1067,23 +1200,32 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   a.page_shift = 31 + l;
   a.page_mul = (uint32_t)(((1ull << (31 + l)) + p->block_size - 1) / (uint64_t)p->block_size);
   const uint64_t rows = (uint64_t)dense.rows * p->n1, keys = (uint64_t)p->key_rows;
-  CUtensorMap q, qr, k64, r64, k16, r16, k1, r1, v32;
+  a.box_keys = 64;
+  while (a.box_keys > 8 && p->block_size % a.box_keys != 0) a.box_keys /= 2;
+  const bool whole = a.box_keys == 64;
+  a.k_group = whole ? 1024 : 2048; a.k_block = whole ? 8192 : 1024;
+  a.v_group = whole ? 1024 : 4096; a.v_block = whole ? 4096 : 1024;
+  CUtensorMap q, qr, kh, rh, k8, r8, k1, r1, vh;
   if (!make_tmap_2d_16bit(&q, p->query, rows, 512, 1024, 64, 64, bf16) ||
       !make_tmap_2d_16bit(&qr, p->query_rope, rows, 64, 128, 64, 64, bf16) ||
-      !spa_tmap_k(&k64, p->key, keys, bf16) ||
-      !make_tmap_2d_16bit(&r64, p->key_rope, keys, 64, 128, 64, 64, bf16) ||
-      !make_tmap_2d_16bit(&k16, p->key, keys, 512, 1024, 16, 64, bf16) ||
-      !make_tmap_2d_16bit(&r16, p->key_rope, keys, 64, 128, 16, 64, bf16) ||
+      !spa_tmap(&kh, p->key, keys, a.box_keys, whole, false, bf16) ||
+      !spa_tmap(&vh, p->key, keys, std::min(a.box_keys, 32), whole, true, bf16) ||
+      !make_tmap_2d_16bit(&k8, p->key, keys, 512, 1024, 8, 64, bf16) ||
+      !make_tmap_2d_16bit(&rh, p->key_rope, keys, 64, 128, a.box_keys, 64, bf16) ||
+      !make_tmap_2d_16bit(&r8, p->key_rope, keys, 64, 128, 8, 64, bf16) ||
       !make_tmap_gather4_16bit(&k1, p->key, keys, 512, 1024, 64, bf16) ||
-      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16) || !spa_tmap_v(&v32, p->key, keys, bf16))
+      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16))
     return DSA_ERR_CUDA;
   if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
-  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, k64, r64, k16, r16,
-                   k1, r1, v32, a) !=
+  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k8, r8,
+                   k1, r1, vh, a) !=
       cudaSuccess)
     return DSA_ERR_CUDA;
-  if (launch_after(spa_join_kernel, dim3(d.rows, (p->n1 + kSpaJoinWarps - 1) / kSpaJoinWarps), dim3(kSpaJoinWarps * 32), 0, st, d,
-                   a.is_bf16) != cudaSuccess)
+  // few rows: four warps each; else a row per warp, or more where there are so many tiles that most are written by their jobs
+  const int32_t per = rows <= 1024 ? 2 : w.own_tiles <= 256 ? 8 : w.own_tiles <= 2048 ? 32 : kSpaRows;
+  const dim3 join_grid((unsigned)w.own_tiles, (unsigned)(kSpaRows / per));
+  if ((rows <= 1024 ? launch_after(spa_join_kernel<4>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, per, a.is_bf16)
+                    : launch_after(spa_join_kernel<1>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, per, a.is_bf16)) != cudaSuccess)
     return DSA_ERR_CUDA;
   count_launch(3);
   if (w.redo_used) {
