@@ -23,9 +23,9 @@
 // 5e-7 of itself after 36 steps, and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
 //
 // Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, as many per box (64, 32, 16, 8) as divide the
-// page size, else (and at the ends of a range, where some of 8 are not wanted) with gather4, four rows each; rows
-// that are not wanted and absent pages are read at a row past the tensor, which gives zeros without touching
-// memory: what lies behind a sequence's end never enters a product.  Bytes are counted on the even CTA's barriers, where
+// page size, else with gather4, four rows each.  Absent pages are read at a row past the tensor, which gives zeros without
+// touching memory, and so are the values behind a sequence's end (gathered where they share a group of 8 with
+// others): 0 x NaN would be NaN.  Keys behind the end only make scores that are masked.  Bytes are counted on the even CTA's barriers, where
 // the products are issued.  Rings: K five units of 64 keys x 128 features (the fifth, the rope, 64), one tile,
 // V three units of 32 keys x 256 columns, refilled unit by unit; P has two buffers.
 //
@@ -63,11 +63,10 @@ constexpr int kSpaSnapTiles = 3;     // tiles that a share may be longer by so t
 constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
 constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
 constexpr uint32_t kSpaBlk = 64 * 128;                      // 64 keys x 64 features
-// Pages of 64 (or multiples): a unit is one box, block after block (K [2 blocks][64 keys][128 bytes], V [4 blocks of columns]
-// [32 keys][128 bytes]).  Other pages: groups of 8 keys (1024 bytes per 64 features, one swizzle atom), all of a group's
-// blocks together, so that a box of 32, 16 or 8 keys is in one piece: K [8 groups][2 blocks][8 keys], V [4 groups][4
-// blocks][8 keys].  The second order costs 1-3 % (attend 64 x 128 heads, pages of 128: 246 -> 253 us), one load per
-// block and 16 keys in the first 25 % (pages of 16: 105 -> 86 us).
+// Keys lie in groups of 8 (1024 bytes per 64 features, one swizzle atom), all of a group's blocks together, so that a box of any
+// multiple of 8 keys is in one piece: K [8 groups][2 blocks][8 keys][128 bytes], V [4 groups][4 blocks of columns][8 keys]
+// [128 bytes].  (Block after block, pages of 16 take a load per block and 16 keys: 105 -> 86 us for 33 x 2 x 64 heads;
+// pages of 64 take the same time either way.)
 constexpr uint32_t kSpaKUnit = 2 * kSpaBlk;                 // 64 keys x 128 features; the fifth unit, the rope, has 64
 constexpr uint32_t kSpaVUnit = 4 * 32 * 128;                // 32 keys x 256 columns
 constexpr uint32_t kSpaPBlk = 64 * 128;                     // 64 rows x 64 keys
@@ -125,7 +124,7 @@ struct SpaDev {
   int32_t* redo_list;       // [rows]
   int32_t* redo_count;
   int32_t* status;
-  float* part_o;            // [slots, 128, 512]
+  float* part_o;            // [slots, 64 groups of 8 columns, 128, 8]: a warp's store of 8 columns is in one piece
   float* part_m;            // [slots, 128] maximum of the scaled scores, log2 units
   float* part_l;            // [slots, 128] sum relative to it; 0: the row takes no part
   // outputs
@@ -406,21 +405,21 @@ struct SpaArgs {
   float scale_log2;
   int32_t is_bf16, key_rows, blocks;
   int32_t box_keys;                // 64, 32, 16 or 8: keys per box
-  int32_t k_group, k_block, v_group, v_block;   // bytes from a group of 8 keys, and from a block of 64 columns, to the next
   uint32_t page_mul, page_shift;   // position / page size = position * page_mul >> page_shift (positions below 2^31)
 };
 
 // Where the positions pos .. pos + 3 of a job (pos a multiple of 4) lie in the cache: the look-ups first, so that they are
-// in flight over the waits of the tile before, the rows when they are needed.  A position that is not
-// wanted (outside lo .. hi - 1) or whose block is absent gets key_rows, a row past the tensor, which is loaded as zeros.
+// in flight over the waits of the tile before, the rows when they are needed.  Positions are wanted within lo .. hi - 1, and,
+// for boxes of n keys that may hold others too, in all of a box that has one of those (n = 1: no others).  A position that is
+// not wanted, or whose block is absent, gets key_rows, a row past the tensor, which is loaded as zeros.
 struct SpaQuad {
   int32_t blk[4], off[4];
-  __device__ __forceinline__ void look_up(const SpaArgs& a, const SpaJob& j, int32_t pos) {
+  __device__ __forceinline__ void look_up(const SpaArgs& a, const SpaJob& j, int32_t pos, int32_t n) {
     const int32_t* table = a.p.seq.block_table + (int64_t)j.table_row * a.p.seq.max_blocks;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t x = pos + i;
-      const bool in = x >= j.lo && x < j.hi;
+      const bool in = (x & -n) + n > j.lo && (x & -n) < j.hi;
       const int32_t page = (int32_t)(((uint64_t)(uint32_t)x * a.page_mul) >> a.page_shift);
       off[i] = in ? x - page * a.p.seq.block_size : -1;
       blk[i] = in ? table[page] : -1;
@@ -438,9 +437,9 @@ __device__ __forceinline__ bool spa_box(const SpaArgs& a, const SpaJob& j, int32
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSpaThreads, 1)
 spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_qr,
                      const __grid_constant__ CUtensorMap tmap_kh, const __grid_constant__ CUtensorMap tmap_rh,
-                     const __grid_constant__ CUtensorMap tmap_k8, const __grid_constant__ CUtensorMap tmap_r8,
                      const __grid_constant__ CUtensorMap tmap_k1, const __grid_constant__ CUtensorMap tmap_r1,
-                     const __grid_constant__ CUtensorMap tmap_vh, const SpaArgs a) {
+                     const __grid_constant__ CUtensorMap tmap_vh, const __grid_constant__ CUtensorMap tmap_v8,
+                     const SpaArgs a) {
   extern __shared__ __align__(1024) unsigned char spa_sm[];
   unsigned char* q_s = spa_sm + kSpaOffQ;
   unsigned char* k_s = spa_sm + kSpaOffK;
@@ -500,24 +499,18 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   } else if (warp == 0 || warp == kSpaKWarp1) {
     // ------------------------------------------------------------------ K loads
     // Two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3.  Lane 2 g + i of the first 16 holds positions
-    // 8 g + 4 i .. + 3 of this CTA's 64.  Boxes are as high as pages allow (64, 32, 16 or 8 keys); where a box would
-    // reach past the wanted positions it is cut into groups of 8, and a group that is cut itself (or every one, where pages
-    // are no multiple of 8) is gathered, four rows a time.  One lane issues: lanes that each issue their own cost 130
-    // cycles a load.
+    // 8 g + 4 i .. + 3 of this CTA's 64.  Boxes are as high as pages allow (64, 32, 16 or 8 keys), and whole even where
+    // only some of their keys are wanted: what the others score is masked.  Pages that are no multiple of 8 are gathered,
+    // four rows a time.  One lane issues: lanes that each issue their own cost 130 cycles a load.
     const uint32_t dst0 = ptx::smem_u32(k_s), bar0 = ptx::map_to_rank(&k_full[0], 0);
     const int u0 = warp == 0 ? 0 : 2, units = warp == 0 ? 3 : 2;
-    const int high = a.box_keys / 8;                   // groups per box
-    const bool dense = a.box_keys == 64;
+    const bool boxes = (a.p.seq.block_size & 7) == 0;
     SpaWalk w;
     w.start(a.p, cluster);
     SpaQuad quad;
-    bool box = false, box8 = false;
     auto look_up = [&]() {
-      if (!w.more()) return;
-      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64 + (lane & 15) * 4;
-      box = spa_box(a, w.j, pos & -a.box_keys, a.box_keys);
-      box8 = spa_box(a, w.j, pos & ~7, 8);
-      quad.look_up(a, w.j, pos);
+      if (w.more())
+        quad.look_up(a, w.j, w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64 + (lane & 15) * 4, boxes ? a.box_keys : 1);
     };
     look_up();
     bool ok = true;
@@ -525,7 +518,6 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int32_t r[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
-      const uint32_t boxes = __ballot_sync(0xffffffffu, box), boxes8 = __ballot_sync(0xffffffffu, box8);
       w.next_tile();
       look_up();
 #pragma unroll 1
@@ -535,46 +527,31 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaKUnit;
         if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[u], u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
+        if (boxes) {
 #pragma unroll 1
-        for (int g = 0; g < 8;) {
-          const int32_t y0 = __shfl_sync(0xffffffffu, r[0], 2 * g);
-          const bool tall = (boxes >> (2 * g)) & 1;
-          if (tall) {
+          for (int g = 0; g < 8; g += a.box_keys / 8) {
+            const int32_t y = __shfl_sync(0xffffffffu, r[0], 2 * g);
             if (lane == 0) {
-              if (u < 4) ptx::tma_load_4d_pair(dst + g * a.k_group, &tmap_kh, bar, u * 128, dense ? y0 : 0, 0, dense ? 0 : (y0 + 7) >> 3);
-              else ptx::tma_load_2d_pair(dst + g * 1024, &tmap_rh, bar, 0, y0);
+              if (u < 4) ptx::tma_load_4d_pair(dst + g * 2048, &tmap_kh, bar, u * 128, 0, 0, (y + 7) >> 3);
+              else ptx::tma_load_2d_pair(dst + g * 1024, &tmap_rh, bar, 0, y);
             }
-            g += high;
-            continue;
           }
-          if ((boxes8 >> (2 * g)) & 1) {
-            if (lane == 0) {
-              if (u < 4) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  ptx::tma_load_2d_pair(dst + g * a.k_group + e * a.k_block, &tmap_k8, bar, u * 128 + e * 64, y0);
-              } else {
-                ptx::tma_load_2d_pair(dst + g * 1024, &tmap_r8, bar, 0, y0);
-              }
-            }
-            ++g;
-            continue;
-          }
+        } else {
 #pragma unroll 1
-          for (int q = 2 * g; q < 2 * g + 2; ++q) {
+          for (int q = 0; q < 16; ++q) {
             const int32_t x0 = __shfl_sync(0xffffffffu, r[0], q), x1 = __shfl_sync(0xffffffffu, r[1], q),
                           x2 = __shfl_sync(0xffffffffu, r[2], q), x3 = __shfl_sync(0xffffffffu, r[3], q);
             if (lane == 0) {
               if (u < 4) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                  ptx::tma_gather4_2d_pair(dst + g * a.k_group + e * a.k_block + (q & 1) * 512, &tmap_k1, bar, u * 128 + e * 64, x0, x1, x2, x3);
+                  ptx::tma_gather4_2d_pair(dst + (q >> 1) * 2048 + e * 1024 + (q & 1) * 512, &tmap_k1, bar, u * 128 + e * 64,
+                                           x0, x1, x2, x3);
               } else {
                 ptx::tma_gather4_2d_pair(dst + q * 512, &tmap_r1, bar, 0, x0, x1, x2, x3);
               }
             }
           }
-          ++g;
         }
         __syncwarp();
       }
@@ -582,11 +559,11 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   } else if (warp == 1 || warp == kSpaVWarp1) {
     // ------------------------------------------------------------------ V loads
     // Two warps, 1 has the units (32 keys x 256 columns) 0 and 2, 15 the units 1 and 3.  Lane 2 g + i holds positions
-    // 8 g + 4 i .. + 3 of the tile's 128; boxes as for K, of up to 32 keys.
+    // 8 g + 4 i .. + 3 of the tile's 128.  Boxes of up to 32 keys; what is not wanted has to be zero here, so that at the ends
+    // of a range a box is cut into groups of 8, and the group that is cut itself is gathered.
     const uint32_t dst0 = ptx::smem_u32(v_s), bar0 = ptx::map_to_rank(&v_full[0], 0);
     const int32_t box_keys = min(a.box_keys, 32);
-    const int high = box_keys / 8;
-    const bool dense = a.box_keys == 64;
+    const int high = box_keys / 8;                     // groups per box
     SpaWalk w;
     w.start(a.p, cluster);
     SpaQuad quad;
@@ -596,7 +573,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + lane * 4;
       box = spa_box(a, w.j, pos & -box_keys, box_keys);
       box8 = spa_box(a, w.j, pos & ~7, 8);
-      quad.look_up(a, w.j, pos);
+      quad.look_up(a, w.j, pos, 1);
     };
     look_up();
     bool ok = true;
@@ -617,23 +594,12 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll 1
         for (int g = 0; g < 4;) {
           const int l = (u * 4 + g) * 2;
-          const int32_t y0 = __shfl_sync(0xffffffffu, r[0], l);
+          const int32_t y = __shfl_sync(0xffffffffu, r[0], l);
           const bool tall = (boxes >> l) & 1;
-          if (tall) {
+          if (tall || ((boxes8 >> l) & 1)) {
             if (lane == 0)
-              ptx::tma_load_5d_pair(dst + g * a.v_group, &tmap_vh, bar, (int32_t)rank * 128, dense ? y0 : 0, 0, 0,
-                                    dense ? 0 : (y0 + 7) >> 3);
-            g += high;
-            continue;
-          }
-          if ((boxes8 >> l) & 1) {
-            if (lane == 0) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                ptx::tma_load_2d_pair(dst + g * a.v_group + c * a.v_block, &tmap_k8, bar,
-                                      (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, y0);
-            }
-            ++g;
+              ptx::tma_load_5d_pair(dst + g * 4096, tall ? &tmap_vh : &tmap_v8, bar, (int32_t)rank * 128, 0, 0, 0, (y + 7) >> 3);
+            g += tall ? high : 1;
             continue;
           }
 #pragma unroll 1
@@ -643,7 +609,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             if (lane == 0) {
 #pragma unroll
               for (int c = 0; c < 4; ++c)
-                ptx::tma_gather4_2d_pair(dst + g * a.v_group + c * a.v_block + q * 512, &tmap_k1, bar,
+                ptx::tma_gather4_2d_pair(dst + g * 4096 + c * 1024 + q * 512, &tmap_k1, bar,
                                          (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
             }
           }
@@ -678,9 +644,9 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
-      const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s), a.k_group);
+      const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s), 2048);
       const uint64_t rd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
-      const uint32_t q_hi = (uint32_t)(qd >> 32), k_block = a.k_block / 16;
+      const uint32_t q_hi = (uint32_t)(qd >> 32);
       const uint32_t tm = tmem + kSpaTmS + (second ? 64 : 0);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
@@ -703,7 +669,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               for (int kk = 0; kk < 8; ++kk)   // (addresses in a descriptor count 16 bytes)
                 if (kk < 4 || u < 4)
                   ptx::mma_ss_pair_lo(tm + b * 128, ql + (kk >> 2) * (kSpaQBlk / 16) + (kk & 3) * 2, q_hi,
-                                      kl + (kk >> 2) * k_block + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
+                                      kl + (kk >> 2) * (1024 / 16) + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
               ptx::mma_commit_pair(&k_empty[u]);
               if (i == units - 1) ptx::mma_commit_pair(&s_full[b]);
             }
@@ -720,9 +686,8 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
-      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), a.v_block, a.v_group);
+      const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 1024, 4096);
       const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
-      const uint32_t v_half = 2 * a.v_block / 16, v_step = 2 * a.v_group / 16;   // two blocks of columns, 16 keys
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
         ok = ptx::mbar_spin_cluster_warp(o_free, (n_job & 1) ^ 1, abort_flag);
@@ -743,7 +708,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * v_half + kk * v_step, v_hi,
+                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (2048 / 16) + kk * (8192 / 16), v_hi,
                                       a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
               ptx::mma_commit_pair(&v_empty[slot]);
               if (u == 3) ptx::mma_commit_pair(&p_empty[n & 1]);
@@ -913,7 +878,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const float total = any ? l_row * ex2(m_ref - m_true) : 0.f;     // relative to the row's maximum
       const int32_t col0 = g * 256 + half * 128;     // this lane's columns
       if (slot >= 0) {
-        float* o_row = a.p.part_o + ((int64_t)slot * kSpaRows + trow) * 512 + col0;
+        float* o_row = a.p.part_o + ((int64_t)slot * 64 + col0 / 8) * (kSpaRows * 8) + trow * 8;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -923,7 +888,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
           if (any) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ptx::st_global_v8(o_row + c * 32 + i * 8, o + i * 8);
+            for (int i = 0; i < 4; ++i) ptx::st_global_v8(o_row + (c * 4 + i) * (kSpaRows * 8), o + i * 8);
           }
         }
         if (g == 0 && half == 0) {
@@ -974,11 +939,12 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 }
 
 // ---- join: the rows whose result is in parts, or that see nothing ----------------------------------
-// A block takes some rows of a row tile: where their parts are is the same for all of them (but for the prefix tile of a packed
-// sequence, one of two), and a tile that its job has written itself is left at once.  kWarps warps join a row, with 2 kWarps
-// parts' loads in flight: one where there are rows enough, four where there are few (8 x 16 heads behind 8192 tokens,
-// where a row has 60 parts: 44 -> 33 us a call; 64 x 128 heads, two parts: 25 us with four, 15 with one).
+// A block works on a row tile: where the parts are is the same for all its rows (but for the prefix tile of a packed sequence,
+// one of two), and a tile that its job has written itself is left at once.  A warp joins 16 columns of 32 rows, a row per
+// lane (8 columns of 32 rows are 1 KB in one piece), with four parts' loads in flight; the warps of a block have the same rows
+// and look the parts' maxima and sums up together, while the first O are on their way.
 constexpr int kSpaJoinThreads = 256;
+constexpr int kSpaJoinBlocks = (kSpaRows / 32) * (512 / 16) / (kSpaJoinThreads / 32);   // blocks of a row tile, a task per warp
 struct SpaParts { int32_t first, count, uncut; };      // first share, number of shares, partial of a job in one share
 __device__ __forceinline__ SpaParts spa_parts(const SpaDev& p, int32_t job, int32_t share) {
   SpaParts w = {0, 0, -1};
@@ -990,8 +956,8 @@ __device__ __forceinline__ SpaParts spa_parts(const SpaDev& p, int32_t job, int3
   }
   return w;
 }
-template <int kWarps>
-__global__ void __launch_bounds__(kSpaJoinThreads, kWarps == 1 ? 3 : 2) spa_join_kernel(const SpaDev p, int32_t rows_per_block, int32_t is_bf16) {
+__global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaDev p, int32_t is_bf16) {
+  __shared__ float2 ml_s[2 * kSpaClusters + 2][32];      // (maximum, sum) of part, row
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31;
@@ -1005,84 +971,78 @@ __global__ void __launch_bounds__(kSpaJoinThreads, kWarps == 1 ? 3 : 2) spa_join
   const int32_t total = min(kSpaRows, tokens * p.n1 - i * kSpaRows), active = min(total, s.act_q * p.n1 - i * kSpaRows);
   const SpaParts own = spa_parts(p, mine.x, share);
   const bool written = own.count == 1 && own.uncut < 0;      // the job wrote its rows itself
-  const int32_t r0 = (int32_t)blockIdx.y * rows_per_block, r1 = min(r0 + rows_per_block, total);
-  if (r0 >= total || (written && r1 <= active)) return;
+  if (total <= 0 || (written && total == active)) return;
   SpaParts pre[2] = {{0, 0, -1}, {0, 0, -1}};
   const int32_t pre0 = row0 / kSpaRows;
   if (s.packed) {
     pre[0] = spa_parts(p, p.place[pre0].x, share);
     if ((row0 + total - 1) / kSpaRows > pre0) pre[1] = spa_parts(p, p.place[pre0 + 1].x, share);
   }
-  constexpr int kCols = 4 / kWarps, kFly = 2 * kWarps;             // groups of four columns per lane; parts in flight
-  const int col = (int)((threadIdx.x >> 5) % kWarps) * 32 + lane;
-  for (int32_t r = r0 + (threadIdx.x >> 5) / kWarps; r < r1; r += kSpaJoinThreads / 32 / kWarps) {
-    if (written && r < active) continue;
-    const int64_t row = row0 + r;
+  const int warp = threadIdx.x >> 5;
+  for (int32_t y = blockIdx.y; y < kSpaJoinBlocks; y += gridDim.y) {
+    const int32_t r = (y >> 2) * 32 + lane, cols = ((y & 3) * 8 + warp) * 16;
+    if ((y >> 2) * 32 >= total) break;
+    const bool todo = r < total && !(written && r < active);
+    const int32_t row = row0 + min(r, total - 1), prow = row % kSpaRows;
     const bool second = row / kSpaRows > pre0;
     const int32_t p_first = second ? pre[1].first : pre[0].first, p_uncut = second ? pre[1].uncut : pre[0].uncut;
-    const int32_t p_count = r < active ? (second ? pre[1].count : pre[0].count) : 0;
-    const int32_t o_count = r < active ? own.count : 0, parts = o_count + p_count;
-    // partial of part k: a job's first share leaves it at 2 c + 1, the later ones at 2 c
-    auto at = [&](int32_t k) -> int64_t {
+    const int32_t p_count = todo && r < active ? (second ? pre[1].count : pre[0].count) : 0;
+    const int32_t o_count = todo && r < active ? own.count : 0, parts = o_count + p_count;
+    // row of the partials for part k: a job's first share leaves it in slot 2 c + 1, the later ones in 2 c
+    auto at = [&](int32_t k, int32_t& tr) -> int64_t {
       const bool o = k < o_count;
       if (!o) k -= o_count;
       const int32_t m = o ? o_count : p_count, c0 = o ? own.first : p_first;
-      const int32_t slot = m == 1 ? (o ? own.uncut : p_uncut) : 2 * (c0 + k) + (k == 0 ? 1 : 0);
-      return (int64_t)slot * kSpaRows + (o ? r : (int32_t)(row % kSpaRows));
+      tr = o ? r : prow;
+      return m == 1 ? (o ? own.uncut : p_uncut) : 2 * (c0 + k) + (k == 0 ? 1 : 0);
     };
-    // the first 32 parts' maxima and sums stay in the lanes
-    float m0 = 0.f, l0 = 0.f, mx = -INFINITY;
-    if (lane < parts) {
-      m0 = p.part_m[at(lane)];
-      l0 = p.part_l[at(lane)];
-      if (l0 != 0.f) mx = m0;
-    }
-    for (int32_t k = lane + 32; k < parts; k += 32)
-      if (p.part_l[at(k)] != 0.f) mx = fmaxf(mx, p.part_m[at(k)]);
+    float v[4][16];
+    auto load = [&](int32_t k0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float4 acc[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-    for (int32_t k0 = 0; k0 < parts; k0 += 32) {
-      float wt = 0.f;
-      if (k0 == 0) wt = l0 != 0.f ? l0 * ex2(m0 - mx) : 0.f;
-      else if (k0 + lane < parts) {
-        const float l = p.part_l[at(k0 + lane)];
-        if (l != 0.f) wt = l * ex2(p.part_m[at(k0 + lane)] - mx);
+      for (int e = 0; e < 4; ++e) {
+        if (k0 + e >= parts) continue;
+        int32_t tr;
+        const int64_t slot = at(k0 + e, tr);
+        const float* o = p.part_o + ((slot * 64 + cols / 8) * kSpaRows + tr) * 8;
+        ptx::ld_global_v8(o, v[e]);
+        ptx::ld_global_v8(o + kSpaRows * 8, v[e] + 8);
       }
-      for (int32_t j0 = 0; j0 < 32 && k0 + j0 < parts; j0 += kFly) {
-        float f[kFly];
-        float4 v[kFly][kCols];
+    };
+    load(0);
+    __syncthreads();               // (the turn before has read ml_s)
+    for (int32_t k = warp; k < parts; k += kSpaJoinThreads / 32) {
+      int32_t tr;
+      const int64_t i = at(k, tr) * kSpaRows + tr;
+      ml_s[k][lane] = make_float2(p.part_m[i], p.part_l[i]);
+    }
+    __syncthreads();
+    float mx = -INFINITY;
+    for (int32_t k = 0; k < parts; ++k) {
+      const float2 ml = ml_s[k][lane];
+      if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
+    }
+    float acc[16] = {}, den = 0.f;
+    for (int32_t k0 = 0; k0 < parts; k0 += 4) {
+      if (k0 > 0) load(k0);
 #pragma unroll
-        for (int e = 0; e < kFly; ++e) {
-          f[e] = __shfl_sync(0xffffffffu, wt, j0 + e);
-          const float4* o = reinterpret_cast<const float4*>(p.part_o + at(k0 + j0 + e) * 512) + col;
+      for (int e = 0; e < 4; ++e) {
+        if (k0 + e >= parts) continue;
+        const float2 ml = ml_s[k0 + e][lane];
+        if (ml.y == 0.f) continue;           // (its O may never have been written)
+        const float f = ml.y * ex2(ml.x - mx);
+        den += f;
 #pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            v[e][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (f[e] != 0.f) v[e][c] = o[c * 32 * kWarps];      // (else O may never have been written)
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kFly; ++e) {
-          den += f[e];
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            acc[c].x += f[e] * v[e][c].x; acc[c].y += f[e] * v[e][c].y;
-            acc[c].z += f[e] * v[e][c].z; acc[c].w += f[e] * v[e][c].w;
-          }
-        }
+        for (int c = 0; c < 16; ++c) acc[c] += f * v[e][c];
       }
     }
+    if (!todo) continue;
     const bool any = den != 0.f;
     const float inv = any ? 1.f / den : 0.f;
-    uint2* out = reinterpret_cast<uint2*>((unsigned char*)p.out + row * 1024) + col;
+    uint32_t out[8];
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
-      out[c * 32 * kWarps] = make_uint2(pack2(acc[c].x * inv, acc[c].y * inv, is_bf16), pack2(acc[c].z * inv, acc[c].w * inv, is_bf16));
-    if (col == 0 && p.softmax_max != nullptr) {
+    for (int c = 0; c < 8; ++c) out[c] = pack2(acc[2 * c] * inv, acc[2 * c + 1] * inv, is_bf16);
+    ptx::st_global_v8((unsigned char*)p.out + (int64_t)row * 1024 + cols * 2, out);
+    if (cols == 0 && p.softmax_max != nullptr) {
       const bool give = p.return_lse && any;
       p.softmax_max[row] = give ? mx * 0.6931471805599453f : 0.f;
       p.softmax_sum[row] = give ? den : 0.f;
@@ -1150,16 +1110,16 @@ inline bool spa_sm100_prepare(int dev) {
   return true;
 }
 
-// The latent cache [keys, 512] as boxes of K units (64 features from 128 u on, both blocks) and of V units (64 columns from 128 c
-// on for CTA c, both blocks of both halves): `box_keys` rows, or as many of them in groups of 8.
-inline bool spa_tmap(CUtensorMap* m, const void* base, uint64_t keys, uint32_t box_keys, bool dense, bool v, bool bf16) {
+// The latent cache [keys, 512] as [keys / 8][2 blocks][8 keys][features] (a box of 64 features from 128 u on, both blocks and n
+// groups is n groups of K unit u), or as [keys / 8][2 halves][2 blocks][8 keys][columns] (64 columns from 128 c on, both
+// blocks of both halves: n groups of a V unit of CTA c).
+inline bool spa_tmap(CUtensorMap* m, const void* base, uint64_t keys, uint32_t box_keys, bool v, bool bf16) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (enc == nullptr) return false;
-  const cuuint64_t rows = dense ? keys : 8, groups = dense ? 1 : std::max<uint64_t>(keys / 8, 1);
-  const cuuint32_t r = dense ? box_keys : 8, g = dense ? 1 : box_keys / 8;
-  const cuuint64_t k_dims[4] = {512, rows, 2, groups}, k_strides[3] = {1024, 128, 8192};
-  const cuuint64_t v_dims[5] = {512, rows, 2, 2, groups}, v_strides[4] = {1024, 128, 512, 8192};
-  const cuuint32_t k_box[4] = {64, r, 2, g}, v_box[5] = {64, r, 2, 2, g}, estr[5] = {1, 1, 1, 1, 1};
+  const cuuint64_t groups = std::max<uint64_t>(keys / 8, 1);
+  const cuuint64_t k_dims[4] = {512, 8, 2, groups}, k_strides[3] = {1024, 128, 8192};
+  const cuuint64_t v_dims[5] = {512, 8, 2, 2, groups}, v_strides[4] = {1024, 128, 512, 8192};
+  const cuuint32_t k_box[4] = {64, 8, 2, box_keys / 8}, v_box[5] = {64, 8, 2, 2, box_keys / 8}, estr[5] = {1, 1, 1, 1, 1};
   return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v ? 5 : 4, const_cast<void*>(base),
              v ? v_dims : k_dims, v ? v_strides : k_strides, v ? v_box : k_box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1202,30 +1162,23 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   const uint64_t rows = (uint64_t)dense.rows * p->n1, keys = (uint64_t)p->key_rows;
   a.box_keys = 64;
   while (a.box_keys > 8 && p->block_size % a.box_keys != 0) a.box_keys /= 2;
-  const bool whole = a.box_keys == 64;
-  a.k_group = whole ? 1024 : 2048; a.k_block = whole ? 8192 : 1024;
-  a.v_group = whole ? 1024 : 4096; a.v_block = whole ? 4096 : 1024;
-  CUtensorMap q, qr, kh, rh, k8, r8, k1, r1, vh;
+  CUtensorMap q, qr, kh, rh, k1, r1, vh, v8;
   if (!make_tmap_2d_16bit(&q, p->query, rows, 512, 1024, 64, 64, bf16) ||
       !make_tmap_2d_16bit(&qr, p->query_rope, rows, 64, 128, 64, 64, bf16) ||
-      !spa_tmap(&kh, p->key, keys, a.box_keys, whole, false, bf16) ||
-      !spa_tmap(&vh, p->key, keys, std::min(a.box_keys, 32), whole, true, bf16) ||
-      !make_tmap_2d_16bit(&k8, p->key, keys, 512, 1024, 8, 64, bf16) ||
+      !spa_tmap(&kh, p->key, keys, a.box_keys, false, bf16) ||
       !make_tmap_2d_16bit(&rh, p->key_rope, keys, 64, 128, a.box_keys, 64, bf16) ||
-      !make_tmap_2d_16bit(&r8, p->key_rope, keys, 64, 128, 8, 64, bf16) ||
       !make_tmap_gather4_16bit(&k1, p->key, keys, 512, 1024, 64, bf16) ||
-      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16))
+      !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16) ||
+      !spa_tmap(&vh, p->key, keys, std::min(a.box_keys, 32), true, bf16) || !spa_tmap(&v8, p->key, keys, 8, true, bf16))
     return DSA_ERR_CUDA;
   if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
-  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k8, r8,
-                   k1, r1, vh, a) !=
+  if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k1, r1,
+                   vh, v8, a) !=
       cudaSuccess)
     return DSA_ERR_CUDA;
-  // few rows: four warps each; else a row per warp, or more where there are so many tiles that most are written by their jobs
-  const int32_t per = rows <= 1024 ? 2 : w.own_tiles <= 256 ? 8 : w.own_tiles <= 2048 ? 32 : kSpaRows;
-  const dim3 join_grid((unsigned)w.own_tiles, (unsigned)(kSpaRows / per));
-  if ((rows <= 1024 ? launch_after(spa_join_kernel<4>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, per, a.is_bf16)
-                    : launch_after(spa_join_kernel<1>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, per, a.is_bf16)) != cudaSuccess)
+  // a task per warp, more where there are so many tiles that most are written by their jobs
+  const dim3 join_grid((unsigned)w.own_tiles, w.own_tiles <= 512 ? kSpaJoinBlocks : 1);
+  if (launch_after(spa_join_kernel, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16) != cudaSuccess)
     return DSA_ERR_CUDA;
   count_launch(3);
   if (w.redo_used) {
