@@ -404,34 +404,198 @@ struct SpaArgs {
   uint32_t idesc_qk, idesc_pv;
   float scale_log2;
   int32_t is_bf16, key_rows, blocks;
-  int32_t box_keys;                // 64, 32, 16 or 8: keys per box
+  int32_t box_keys;                // 64, 32, 16 or 8 keys per box; 0: pages that are no multiple of 8 are gathered
   uint32_t page_mul, page_shift;   // position / page size = position * page_mul >> page_shift (positions below 2^31)
 };
 
-// Where the positions pos .. pos + 3 of a job (pos a multiple of 4) lie in the cache: the look-ups first, so that they are
-// in flight over the waits of the tile before, the rows when they are needed.  Positions are wanted within lo .. hi - 1, and,
-// for boxes of n keys that may hold others too, in all of a box that has one of those (n = 1: no others).  A position that is
-// not wanted, or whose block is absent, gets key_rows, a row past the tensor, which is loaded as zeros.
-struct SpaQuad {
-  int32_t blk[4], off[4];
-  __device__ __forceinline__ void look_up(const SpaArgs& a, const SpaJob& j, int32_t pos, int32_t n) {
-    const int32_t* table = a.p.seq.block_table + (int64_t)j.table_row * a.p.seq.max_blocks;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int32_t x = pos + i;
-      const bool in = (x & -n) + n > j.lo && (x & -n) < j.hi;
-      const int32_t page = (int32_t)(((uint64_t)(uint32_t)x * a.page_mul) >> a.page_shift);
-      off[i] = in ? x - page * a.p.seq.block_size : -1;
-      blk[i] = in ? table[page] : -1;
-    }
+// Where a position of a job lies in the cache: the look-up first, so that it is in flight over the waits of the tile before, the
+// row when it is needed.  A position that is not wanted, or whose block is absent, gets key_rows, a row past the tensor,
+// which is loaded as zeros.
+struct SpaSpot {
+  int32_t blk, off;
+  __device__ __forceinline__ void look_up(const SpaArgs& a, const SpaJob& j, int32_t pos, bool wanted) {
+    const int32_t page = (int32_t)(((uint64_t)(uint32_t)pos * a.page_mul) >> a.page_shift);
+    off = pos - page * a.p.seq.block_size;
+    blk = wanted ? a.p.seq.block_table[(int64_t)j.table_row * a.p.seq.max_blocks + page] : -1;
   }
-  __device__ __forceinline__ int32_t row(const SpaArgs& a, int i) const {
-    return blk[i] >= 0 && blk[i] < a.blocks ? blk[i] * a.p.seq.block_size + off[i] : a.key_rows;
+  __device__ __forceinline__ int32_t row(const SpaArgs& a) const {
+    return blk >= 0 && blk < a.blocks ? blk * a.p.seq.block_size + off : a.key_rows;
   }
 };
-// Are n positions from pos on (a multiple of n) one box of rows: in one page and all wanted, or none of them wanted?
-__device__ __forceinline__ bool spa_box(const SpaArgs& a, const SpaJob& j, int32_t pos, int32_t n) {
-  return pos + n <= j.lo || pos >= j.hi || ((a.p.seq.block_size & (n - 1)) == 0 && pos >= j.lo && pos + n <= j.hi);
+// A warp's loads: who it loads for, and where to.
+struct SpaLoads {
+  const CUtensorMap *box, *box8, *rope, *gather, *rope_gather;
+  uint64_t *full, *empty;
+  uint32_t full_lead;          // full[0] of the even CTA
+  uint32_t dst;
+  int32_t rank, cluster;
+  int32_t u0;                  // first unit
+  volatile int* abort_flag;
+};
+
+// K, pages that are multiples of 8: kBoxes boxes of 64 / kBoxes keys per unit, whole even where only some of their keys are wanted
+// (what the others score is masked).  One thread: a load takes uniform operands, and a tile is a handful of them.
+template <int kBoxes>
+__device__ __forceinline__ void spa_k_boxes(const SpaArgs& a, const SpaLoads& o) {
+  constexpr int kKeys = 64 / kBoxes;
+  SpaWalk w;
+  w.start(a.p, o.cluster);
+  SpaSpot spot[kBoxes];
+  auto look_up = [&]() {
+    if (!w.more()) return;
+    const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + o.rank * 64;
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b) {
+      const int32_t x = pos + b * kKeys;
+      spot[b].look_up(a, w.j, x, x + kKeys > w.j.lo && x < w.j.hi);
+    }
+  };
+  look_up();
+  for (uint32_t n = 0; w.more(); ++n) {
+    int32_t y[kBoxes];
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b) y[b] = spot[b].row(a);
+    w.next_tile();
+    look_up();
+    auto unit = [&](int u) -> bool {
+      if (!ptx::mbar_spin(&o.empty[u], (n & 1) ^ 1, o.abort_flag)) return false;
+      if (o.rank == 0) ptx::mbar_arrive_expect_tx(&o.full[u], 2 * kSpaKUnit);
+#pragma unroll
+      for (int b = 0; b < kBoxes; ++b)
+        ptx::tma_load_4d_pair(o.dst + u * kSpaKUnit + b * (kKeys / 8) * 2048, o.box, o.full_lead + u * 8, u * 128, 0, 0, (y[b] + 7) >> 3);
+      return true;
+    };
+    if (!unit(o.u0) || !unit(o.u0 + 1)) return;
+    if (o.u0 != 0) continue;
+    if (!ptx::mbar_spin(&o.empty[4], (n & 1) ^ 1, o.abort_flag)) return;
+    if (o.rank == 0) ptx::mbar_arrive_expect_tx(&o.full[4], kSpaKUnit);
+#pragma unroll
+    for (int b = 0; b < kBoxes; ++b)
+      ptx::tma_load_2d_pair(o.dst + 4 * kSpaKUnit + b * (kKeys / 8) * 1024, o.rope, o.full_lead + 32, 0, y[b]);
+  }
+}
+
+// V, pages that are multiples of 8: kBoxes boxes of 32 / kBoxes keys per unit.  What is not wanted has to be zero here: where a
+// box would hold some of it, the unit is loaded in groups of 8, and a group that is cut itself is gathered.
+template <int kBoxes>
+__device__ __forceinline__ void spa_v_boxes(const SpaArgs& a, const SpaLoads& o) {
+  constexpr int kKeys = 32 / kBoxes;
+  SpaWalk w;
+  w.start(a.p, o.cluster);
+  SpaSpot spot[2][kBoxes];
+  int32_t first = 0, lo = 0, hi = 0;          // position of the tile, and what is wanted
+  auto look_up = [&]() {
+    if (!w.more()) return;
+    const int32_t pos = w.j.key0 + w.tile() * kSpaKeys;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int b = 0; b < kBoxes; ++b) {
+        const int32_t x = pos + (o.u0 + 2 * i) * 32 + b * kKeys;
+        spot[i][b].look_up(a, w.j, x, x + kKeys > w.j.lo && x < w.j.hi);
+      }
+  };
+  look_up();
+  for (uint32_t n = 0; w.more(); ++n) {
+    int32_t y[2][kBoxes];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int b = 0; b < kBoxes; ++b) y[i][b] = spot[i][b].row(a);
+    first = w.j.key0 + w.tile() * kSpaKeys; lo = w.j.lo; hi = w.j.hi;
+    w.next_tile();
+    look_up();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = n * 4 + o.u0 + 2 * i, use = v / kSpaVUnits, slot = v - use * kSpaVUnits;
+      const int32_t pos = first + (o.u0 + 2 * i) * 32;
+      if (!ptx::mbar_spin(&o.empty[slot], (use & 1) ^ 1, o.abort_flag)) return;
+      if (o.rank == 0) ptx::mbar_arrive_expect_tx(&o.full[slot], 2 * kSpaVUnit);
+      const uint32_t dst = o.dst + slot * kSpaVUnit, bar = o.full_lead + slot * 8;
+      if (pos >= lo && pos + 32 <= hi) {
+#pragma unroll
+        for (int b = 0; b < kBoxes; ++b)
+          ptx::tma_load_5d_pair(dst + b * (kKeys / 8) * 4096, o.box, bar, o.rank * 128, 0, 0, 0, (y[i][b] + 7) >> 3);
+        continue;
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int32_t x = pos + g * 8, row = y[i][g * kBoxes / 4] == a.key_rows ? a.key_rows : y[i][g * kBoxes / 4] + (g * 8) % kKeys;
+        if ((x >= lo && x + 8 <= hi) || x + 8 <= lo || x >= hi) {
+          const int32_t yy = x >= lo && x < hi ? row : a.key_rows;
+          ptx::tma_load_5d_pair(dst + g * 4096, o.box8, bar, o.rank * 128, 0, 0, 0, (yy + 7) >> 3);
+          continue;
+        }
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {
+          int32_t z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t k = q * 4 + e;
+            z[e] = x + k >= lo && x + k < hi && row != a.key_rows ? row + k : a.key_rows;
+          }
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c)
+            ptx::tma_gather4_2d_pair(dst + g * 4096 + c * 1024 + q * 512, o.gather, bar, (c >> 1) * 256 + o.rank * 128 + (c & 1) * 64,
+                                     z[0], z[1], z[2], z[3]);
+        }
+      }
+    }
+  }
+}
+
+// Pages that are no multiple of 8: rows are gathered, four a load.  Lane i holds the positions 4 i .. 4 i + 3 of the CTA's 64 (K) or
+// of the tile's 128 (V); one lane issues (lanes that each issue their own cost 130 cycles a load).
+template <bool kV>
+__device__ __forceinline__ void spa_gather(const SpaArgs& a, const SpaLoads& o) {
+  const int lane = threadIdx.x & 31;
+  SpaWalk w;
+  w.start(a.p, o.cluster);
+  SpaSpot spot[4];
+  auto look_up = [&]() {
+    if (!w.more()) return;
+    const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + (kV ? lane * 4 : o.rank * 64 + (lane & 15) * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) spot[i].look_up(a, w.j, pos + i, pos + i >= w.j.lo && pos + i < w.j.hi);
+  };
+  look_up();
+  for (uint32_t n = 0; w.more(); ++n) {
+    int32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = spot[i].row(a);
+    w.next_tile();
+    look_up();
+    const int units = kV || o.u0 != 0 ? 2 : 3;
+#pragma unroll 1
+    for (int i = 0; i < units; ++i) {
+      const int u = kV ? o.u0 + 2 * i : i == 2 ? 4 : o.u0 + i;
+      const uint32_t use = kV ? (n * 4 + u) / kSpaVUnits : n, slot = kV ? n * 4 + u - use * kSpaVUnits : u;
+      if (!ptx::mbar_spin_warp(&o.empty[slot], (use & 1) ^ 1, o.abort_flag)) return;
+      if (o.rank == 0 && lane == 0)
+        ptx::mbar_arrive_expect_tx(&o.full[slot], kV ? 2 * kSpaVUnit : u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
+      const uint32_t dst = o.dst + slot * (kV ? kSpaVUnit : kSpaKUnit), bar = o.full_lead + slot * 8;
+#pragma unroll 1
+      for (int q = 0; q < (kV ? 8 : 16); ++q) {
+        const int l = kV ? u * 8 + q : q;
+        const int32_t x0 = __shfl_sync(0xffffffffu, r[0], l), x1 = __shfl_sync(0xffffffffu, r[1], l),
+                      x2 = __shfl_sync(0xffffffffu, r[2], l), x3 = __shfl_sync(0xffffffffu, r[3], l);
+        if (lane != 0) continue;
+        if (kV) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            ptx::tma_gather4_2d_pair(dst + (q >> 1) * 4096 + c * 1024 + (q & 1) * 512, o.gather, bar,
+                                     (c >> 1) * 256 + o.rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
+        } else if (u < 4) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            ptx::tma_gather4_2d_pair(dst + (q >> 1) * 2048 + e * 1024 + (q & 1) * 512, o.gather, bar, u * 128 + e * 64, x0, x1, x2, x3);
+        } else {
+          ptx::tma_gather4_2d_pair(dst + q * 512, o.rope_gather, bar, 0, x0, x1, x2, x3);
+        }
+      }
+      __syncwarp();
+    }
+  }
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSpaThreads, 1)
@@ -498,125 +662,30 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     // nothing started
   } else if (warp == 0 || warp == kSpaKWarp1) {
     // ------------------------------------------------------------------ K loads
-    // Two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3.  Lane 2 g + i of the first 16 holds positions
-    // 8 g + 4 i .. + 3 of this CTA's 64.  Boxes are as high as pages allow (64, 32, 16 or 8 keys), and whole even where
-    // only some of their keys are wanted: what the others score is masked.  Pages that are no multiple of 8 are gathered,
-    // four rows a time.  One lane issues: lanes that each issue their own cost 130 cycles a load.
-    const uint32_t dst0 = ptx::smem_u32(k_s), bar0 = ptx::map_to_rank(&k_full[0], 0);
-    const int u0 = warp == 0 ? 0 : 2, units = warp == 0 ? 3 : 2;
-    const bool boxes = (a.p.seq.block_size & 7) == 0;
-    SpaWalk w;
-    w.start(a.p, cluster);
-    SpaQuad quad;
-    auto look_up = [&]() {
-      if (w.more())
-        quad.look_up(a, w.j, w.j.key0 + w.tile() * kSpaKeys + (int32_t)rank * 64 + (lane & 15) * 4, boxes ? a.box_keys : 1);
-    };
-    look_up();
-    bool ok = true;
-    for (uint32_t n = 0; w.more() && ok; ++n) {
-      int32_t r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
-      w.next_tile();
-      look_up();
-#pragma unroll 1
-      for (int i = 0; i < units; ++i) {
-        const int u = i == 2 ? 4 : u0 + i;
-        ok = ptx::mbar_spin_warp(&k_empty[u], (n & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        const uint32_t bar = bar0 + u * 8, dst = dst0 + u * kSpaKUnit;
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&k_full[u], u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
-        if (boxes) {
-#pragma unroll 1
-          for (int g = 0; g < 8; g += a.box_keys / 8) {
-            const int32_t y = __shfl_sync(0xffffffffu, r[0], 2 * g);
-            if (lane == 0) {
-              if (u < 4) ptx::tma_load_4d_pair(dst + g * 2048, &tmap_kh, bar, u * 128, 0, 0, (y + 7) >> 3);
-              else ptx::tma_load_2d_pair(dst + g * 1024, &tmap_rh, bar, 0, y);
-            }
-          }
-        } else {
-#pragma unroll 1
-          for (int q = 0; q < 16; ++q) {
-            const int32_t x0 = __shfl_sync(0xffffffffu, r[0], q), x1 = __shfl_sync(0xffffffffu, r[1], q),
-                          x2 = __shfl_sync(0xffffffffu, r[2], q), x3 = __shfl_sync(0xffffffffu, r[3], q);
-            if (lane == 0) {
-              if (u < 4) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  ptx::tma_gather4_2d_pair(dst + (q >> 1) * 2048 + e * 1024 + (q & 1) * 512, &tmap_k1, bar, u * 128 + e * 64,
-                                           x0, x1, x2, x3);
-              } else {
-                ptx::tma_gather4_2d_pair(dst + q * 512, &tmap_r1, bar, 0, x0, x1, x2, x3);
-              }
-            }
-          }
-        }
-        __syncwarp();
-      }
+    // two warps: 0 has the units 0, 1 and the rope, 14 the units 2 and 3
+    SpaLoads o;
+    o.box = &tmap_kh; o.box8 = nullptr; o.rope = &tmap_rh; o.gather = &tmap_k1; o.rope_gather = &tmap_r1;
+    o.full = k_full; o.empty = k_empty; o.full_lead = ptx::map_to_rank(&k_full[0], 0);
+    o.dst = ptx::smem_u32(k_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 0 ? 0 : 2; o.abort_flag = abort_flag;
+    if (a.box_keys == 0) spa_gather<false>(a, o);
+    else if (lane == 0) {
+      if (a.box_keys == 64) spa_k_boxes<1>(a, o);
+      else if (a.box_keys == 32) spa_k_boxes<2>(a, o);
+      else if (a.box_keys == 16) spa_k_boxes<4>(a, o);
+      else spa_k_boxes<8>(a, o);
     }
   } else if (warp == 1 || warp == kSpaVWarp1) {
     // ------------------------------------------------------------------ V loads
-    // Two warps, 1 has the units (32 keys x 256 columns) 0 and 2, 15 the units 1 and 3.  Lane 2 g + i holds positions
-    // 8 g + 4 i .. + 3 of the tile's 128.  Boxes of up to 32 keys; what is not wanted has to be zero here, so that at the ends
-    // of a range a box is cut into groups of 8, and the group that is cut itself is gathered.
-    const uint32_t dst0 = ptx::smem_u32(v_s), bar0 = ptx::map_to_rank(&v_full[0], 0);
-    const int32_t box_keys = min(a.box_keys, 32);
-    const int high = box_keys / 8;                     // groups per box
-    SpaWalk w;
-    w.start(a.p, cluster);
-    SpaQuad quad;
-    bool box = false, box8 = false;
-    auto look_up = [&]() {
-      if (!w.more()) return;
-      const int32_t pos = w.j.key0 + w.tile() * kSpaKeys + lane * 4;
-      box = spa_box(a, w.j, pos & -box_keys, box_keys);
-      box8 = spa_box(a, w.j, pos & ~7, 8);
-      quad.look_up(a, w.j, pos, 1);
-    };
-    look_up();
-    bool ok = true;
-    for (uint32_t n = 0; w.more() && ok; ++n) {
-      int32_t r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = quad.row(a, i);
-      const uint32_t boxes = __ballot_sync(0xffffffffu, box), boxes8 = __ballot_sync(0xffffffffu, box8);
-      w.next_tile();
-      look_up();
-#pragma unroll 1
-      for (int u = warp == 1 ? 0 : 1; u < 4; u += 2) {
-        const uint32_t v = n * 4 + u, use = v / kSpaVUnits, slot = v - use * kSpaVUnits;
-        ok = ptx::mbar_spin_warp(&v_empty[slot], (use & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        const uint32_t bar = bar0 + slot * 8, dst = dst0 + slot * kSpaVUnit;
-        if (rank == 0 && lane == 0) ptx::mbar_arrive_expect_tx(&v_full[slot], 2 * kSpaVUnit);
-#pragma unroll 1
-        for (int g = 0; g < 4;) {
-          const int l = (u * 4 + g) * 2;
-          const int32_t y = __shfl_sync(0xffffffffu, r[0], l);
-          const bool tall = (boxes >> l) & 1;
-          if (tall || ((boxes8 >> l) & 1)) {
-            if (lane == 0)
-              ptx::tma_load_5d_pair(dst + g * 4096, tall ? &tmap_vh : &tmap_v8, bar, (int32_t)rank * 128, 0, 0, 0, (y + 7) >> 3);
-            g += tall ? high : 1;
-            continue;
-          }
-#pragma unroll 1
-          for (int q = 0; q < 2; ++q) {
-            const int32_t x0 = __shfl_sync(0xffffffffu, r[0], l + q), x1 = __shfl_sync(0xffffffffu, r[1], l + q),
-                          x2 = __shfl_sync(0xffffffffu, r[2], l + q), x3 = __shfl_sync(0xffffffffu, r[3], l + q);
-            if (lane == 0) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                ptx::tma_gather4_2d_pair(dst + g * 4096 + c * 1024 + q * 512, &tmap_k1, bar,
-                                         (c >> 1) * 256 + (int32_t)rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
-            }
-          }
-          ++g;
-        }
-        __syncwarp();
-      }
+    // two warps: 1 has the units 0 and 2, 15 the units 1 and 3
+    SpaLoads o;
+    o.box = &tmap_vh; o.box8 = &tmap_v8; o.rope = nullptr; o.gather = &tmap_k1; o.rope_gather = nullptr;
+    o.full = v_full; o.empty = v_empty; o.full_lead = ptx::map_to_rank(&v_full[0], 0);
+    o.dst = ptx::smem_u32(v_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 1 ? 0 : 1; o.abort_flag = abort_flag;
+    if (a.box_keys == 0) spa_gather<true>(a, o);
+    else if (lane == 0) {
+      if (a.box_keys >= 32) spa_v_boxes<1>(a, o);
+      else if (a.box_keys == 16) spa_v_boxes<2>(a, o);
+      else spa_v_boxes<4>(a, o);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ Q loads
@@ -1161,15 +1230,17 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   a.page_mul = (uint32_t)(((1ull << (31 + l)) + p->block_size - 1) / (uint64_t)p->block_size);
   const uint64_t rows = (uint64_t)dense.rows * p->n1, keys = (uint64_t)p->key_rows;
   a.box_keys = 64;
-  while (a.box_keys > 8 && p->block_size % a.box_keys != 0) a.box_keys /= 2;
+  while (a.box_keys >= 8 && p->block_size % a.box_keys != 0) a.box_keys /= 2;
+  if (a.box_keys < 8) a.box_keys = 0;
+  const uint32_t box_keys = std::max(a.box_keys, 8);
   CUtensorMap q, qr, kh, rh, k1, r1, vh, v8;
   if (!make_tmap_2d_16bit(&q, p->query, rows, 512, 1024, 64, 64, bf16) ||
       !make_tmap_2d_16bit(&qr, p->query_rope, rows, 64, 128, 64, 64, bf16) ||
-      !spa_tmap(&kh, p->key, keys, a.box_keys, false, bf16) ||
-      !make_tmap_2d_16bit(&rh, p->key_rope, keys, 64, 128, a.box_keys, 64, bf16) ||
+      !spa_tmap(&kh, p->key, keys, box_keys, false, bf16) ||
+      !make_tmap_2d_16bit(&rh, p->key_rope, keys, 64, 128, box_keys, 64, bf16) ||
       !make_tmap_gather4_16bit(&k1, p->key, keys, 512, 1024, 64, bf16) ||
       !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16) ||
-      !spa_tmap(&vh, p->key, keys, std::min(a.box_keys, 32), true, bf16) || !spa_tmap(&v8, p->key, keys, 8, true, bf16))
+      !spa_tmap(&vh, p->key, keys, std::min(box_keys, 32u), true, bf16) || !spa_tmap(&v8, p->key, keys, 8, true, bf16))
     return DSA_ERR_CUDA;
   if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
   if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k1, r1,
