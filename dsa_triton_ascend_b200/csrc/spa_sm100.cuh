@@ -178,37 +178,43 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
   __shared__ unsigned long long best_s[32];
   __shared__ int32_t sum_s[3][33];
   __shared__ int32_t total_s[3];
-  __shared__ int32_t tiles_s[kSpaClusters];   // tiles of the first jobs
+  __shared__ int32_t tiles_s[kSpaClusters], place_s[kSpaClusters];   // of the first jobs: tiles, and their place
+  const int nt = blockDim.x, warps = nt >> 5;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dep_launch();
   grid_dep_wait();
   if (tid < 64) p.status[tid] = 0;
   if (p.redo != nullptr) {
     if (tid == 0) *p.redo_count = 0;
-    for (int32_t i = tid; i < p.rows; i += kSpaPlanThreads) p.redo[i] = 0;
+    for (int32_t i = tid; i < p.rows; i += nt) p.redo[i] = 0;
   }
   // the longest sequence (the first of them) lends its pages for the prefix
-  unsigned long long best = 0;
-  for (int32_t b = tid; b < p.seq.batch; b += kSpaPlanThreads) {
-    const int32_t k = max(0, min(p.seq.seq_k[b], p.seq.s2));
-    best = max(best, ((unsigned long long)(uint32_t)k << 32) | (uint32_t)(0x7FFFFFFF - b));
+  int32_t prefix = 0, ref = 0;
+  if (p.pack_rows > 0) {
+    unsigned long long best = 0;
+    for (int32_t b = tid; b < p.seq.batch; b += nt) {
+      const int32_t k = max(0, min(p.seq.seq_k[b], p.seq.s2));
+      best = max(best, ((unsigned long long)(uint32_t)k << 32) | (uint32_t)(0x7FFFFFFF - b));
+    }
+    const int32_t asked = p.prefix_device ? *p.prefix_device : p.prefix;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) best_s[warp] = best;
+    __syncthreads();
+    best = lane < warps ? best_s[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    ref = 0x7FFFFFFF - (int32_t)(uint32_t)best;
+    prefix = max(0, min(asked, (int32_t)(best >> 32)));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) best_s[warp] = best;
-  __syncthreads();
-  best = best_s[lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  const int32_t longest = (int32_t)(best >> 32), ref = 0x7FFFFFFF - (int32_t)(uint32_t)best;
-  int32_t prefix = p.prefix_device ? *p.prefix_device : p.prefix;
-  prefix = max(0, min(prefix, longest));
 
   const int32_t places = p.prefix_tiles + p.own_tiles, rows = p.rows * p.n1;
   int32_t jobs = 0, tiles = 0, packed = 0;   // listed so far
-  for (int32_t f0 = 0; f0 < places; f0 += kSpaPlanThreads) {
+  SpaJob j;
+  int32_t mine = -1;                         // this thread's job of the last turn
+  for (int32_t f0 = 0; f0 < places; f0 += nt) {
     const int32_t f = f0 + tid;
-    SpaJob j;
+    mine = -1;
     j.tiles = 0;
     j.slot = -1;
     int32_t of_seq = 0;
@@ -279,14 +285,14 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     }
     __syncthreads();
     if (warp < 3) {
-      const int32_t mine = sum_s[warp][lane];
-      int32_t z = mine;
+      const int32_t in = lane < warps ? sum_s[warp][lane] : 0;
+      int32_t z = in;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int32_t y = __shfl_up_sync(0xffffffffu, z, o);
         if (lane >= o) z += y;
       }
-      sum_s[warp][lane] = z - mine;
+      sum_s[warp][lane] = z - in;
       if (lane == 31) total_s[warp] = z;
     }
     __syncthreads();
@@ -297,6 +303,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
         j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1];
         if (v[2]) j.slot = 2 * p.clusters + packed + sum_s[2][warp] + x[2] - v[2];
         p.job[at] = j;
+        mine = at;
         if (at < kSpaClusters) tiles_s[at] = j.tiles;
       }
     }
@@ -324,14 +331,14 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
       if (warp == 0) {
         int32_t before = 0;
         for (int32_t i0 = 0; i0 < jobs; i0 += 32) {
-          const int32_t i = i0 + lane, mine = i < jobs ? (tiles_s[i] + share - 1) / share : 0;
-          int32_t z = mine;
+          const int32_t i = i0 + lane, mine_parts = i < jobs ? (tiles_s[i] + share - 1) / share : 0;
+          int32_t z = mine_parts;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const int32_t y = __shfl_up_sync(0xffffffffu, z, o);
             if (lane >= o) z += y;
           }
-          if (i < jobs) p.job[i].tile0 = (before + z - mine) * share;
+          if (i < jobs) place_s[i] = (before + z - mine_parts) * share;
           before += __shfl_sync(0xffffffffu, z, 31);
         }
         if (lane == 0) total_s[1] = before * share;
@@ -344,18 +351,30 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     p.plan->share = share;
     p.plan->prefix = prefix;
   }
-  for (int32_t c = tid; c < p.clusters; c += kSpaPlanThreads)
+  for (int32_t c = tid; c < p.clusters; c += nt)
     if ((int64_t)c * share >= tiles) p.start[c].at = p.start[c].end = 0;
-  for (int32_t i = tid; i < jobs; i += kSpaPlanThreads) {
+  auto deal = [&](int32_t i) {               // job i = j: its place, and the pairs that begin in it
+    if (single) {
+      j.tile0 = place_s[i];
+      p.job[i].tile0 = j.tile0;
+    }
     SpaStart w;
-    w.j = p.job[i];
+    w.j = j;
     w.index = i;
     w.unused = 0;
-    const int32_t t1 = w.j.tile0 + w.j.tiles;
-    for (int32_t c = (w.j.tile0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
+    const int32_t t1 = j.tile0 + j.tiles;
+    for (int32_t c = (j.tile0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
       w.at = c * share;
       w.end = min(w.at + share, single ? t1 : tiles);
       p.start[c] = w;
+    }
+  };
+  if (places <= nt) {                        // (the jobs are still at hand)
+    if (mine >= 0) deal(mine);
+  } else {
+    for (int32_t i = tid; i < jobs; i += nt) {
+      j = p.job[i];
+      deal(i);
     }
   }
 }
@@ -668,7 +687,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     o.full = k_full; o.empty = k_empty; o.full_lead = ptx::map_to_rank(&k_full[0], 0);
     o.dst = ptx::smem_u32(k_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 0 ? 0 : 2; o.abort_flag = abort_flag;
     if (a.box_keys == 0) spa_gather<false>(a, o);
-    else if (lane == 0) {
+    else if (ptx::elect_one()) {
       if (a.box_keys == 64) spa_k_boxes<1>(a, o);
       else if (a.box_keys == 32) spa_k_boxes<2>(a, o);
       else if (a.box_keys == 16) spa_k_boxes<4>(a, o);
@@ -682,7 +701,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     o.full = v_full; o.empty = v_empty; o.full_lead = ptx::map_to_rank(&v_full[0], 0);
     o.dst = ptx::smem_u32(v_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 1 ? 0 : 1; o.abort_flag = abort_flag;
     if (a.box_keys == 0) spa_gather<true>(a, o);
-    else if (lane == 0) {
+    else if (ptx::elect_one()) {
       if (a.box_keys >= 32) spa_v_boxes<1>(a, o);
       else if (a.box_keys == 16) spa_v_boxes<2>(a, o);
       else spa_v_boxes<4>(a, o);
@@ -706,8 +725,9 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
   } else if (warp == kSpaQkWarp0 || warp == kSpaQkWarp1) {
     // ------------------------------------------------------------------ QK^T issuers
-    // Two, each with its feature blocks and its partial score.  The loop is warp-uniform, one elected lane issues.
-    if (rank == 0) {
+    // Two, each with its units and its partial score.  (One elected thread: chosen by its number in place of elect, it takes twice
+    // as long per product; a warp-uniform loop 2 % of the whole.)
+    if (rank == 0 && ptx::elect_one()) {
       const bool second = warp == kSpaQkWarp1;      // units 2 and 3; the first: 0, 1 and the rope
       const int units = second ? 2 : 3;
       SpaWalk w;
@@ -719,39 +739,35 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const uint32_t tm = tmem + kSpaTmS + (second ? 64 : 0);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
-        ok = ptx::mbar_spin_warp(q_full, n_job & 1, abort_flag);
+        ok = ptx::mbar_spin(q_full, n_job & 1, abort_flag);
         const int32_t stop = w.stop();
         for (int32_t t = w.tile(); t < stop && ok; ++t, ++n) {
           const uint32_t b = n & 1;
-          ok = ptx::mbar_spin_cluster_warp(&s_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
+          ok = ptx::mbar_spin_cluster(&s_empty[b], ((n >> 1) & 1) ^ 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int i = 0; i < units; ++i) {
             const int u = second ? 2 + i : (i == 2 ? 4 : i);
-            ok = ptx::mbar_spin_warp(&k_full[u], n & 1, abort_flag);
+            ok = ptx::mbar_spin(&k_full[u], n & 1, abort_flag);
             if (!ok) break;
-            if (ptx::elect_one()) {
-              const uint32_t ql = (uint32_t)qd + u * (2 * kSpaQBlk / 16), kl = (uint32_t)kd + u * (kSpaKUnit / 16);
-              const uint32_t k_hi = (uint32_t)((u < 4 ? kd : rd) >> 32);
+            const uint32_t ql = (uint32_t)qd + u * (2 * kSpaQBlk / 16), kl = (uint32_t)kd + u * (kSpaKUnit / 16);
+            const uint32_t k_hi = (uint32_t)((u < 4 ? kd : rd) >> 32);
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)   // (addresses in a descriptor count 16 bytes)
-                if (kk < 4 || u < 4)
-                  ptx::mma_ss_pair_lo(tm + b * 128, ql + (kk >> 2) * (kSpaQBlk / 16) + (kk & 3) * 2, q_hi,
-                                      kl + (kk >> 2) * (1024 / 16) + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
-              ptx::mma_commit_pair(&k_empty[u]);
-              if (i == units - 1) ptx::mma_commit_pair(&s_full[b]);
-            }
-            __syncwarp();
+            for (int kk = 0; kk < 8; ++kk)   // (addresses in a descriptor count 16 bytes)
+              if (kk < 4 || u < 4)
+                ptx::mma_ss_pair_lo(tm + b * 128, ql + (kk >> 2) * (kSpaQBlk / 16) + (kk & 3) * 2, q_hi,
+                                    kl + (kk >> 2) * (1024 / 16) + (kk & 3) * 2, k_hi, a.idesc_qk, (i > 0 || kk > 0) ? 1u : 0u);
+            ptx::mma_commit_pair(&k_empty[u]);
+            if (i == units - 1) ptx::mma_commit_pair(&s_full[b]);
           }
         }
-        if (ok && ptx::elect_one()) ptx::mma_commit_pair(q_empty);
-        __syncwarp();
+        if (ok) ptx::mma_commit_pair(q_empty);
       }
     }
   } else if (warp == kSpaPvWarp) {
     // ------------------------------------------------------------------ PV issuer
-    if (rank == 0) {
+    if (rank == 0 && ptx::elect_one()) {
       SpaWalk w;
       w.start(a.p, cluster);
       bool ok = true;
@@ -759,30 +775,27 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
       uint32_t n = 0;
       for (uint32_t n_job = 0; w.more() && ok; ++n_job, w.next_job()) {
-        ok = ptx::mbar_spin_cluster_warp(o_free, (n_job & 1) ^ 1, abort_flag);
+        ok = ptx::mbar_spin_cluster(o_free, (n_job & 1) ^ 1, abort_flag);
         const int32_t first = w.tile(), stop = w.stop();
         for (int32_t t = first; t < stop && ok; ++t, ++n) {
-          ok = ptx::mbar_spin_cluster_warp(&p_full[n & 1], (n >> 1) & 1, abort_flag);
+          ok = ptx::mbar_spin_cluster(&p_full[n & 1], (n >> 1) & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int u = 0; u < 4; ++u) {
             const uint32_t v = n * 4 + u, use = v / kSpaVUnits, slot = v - use * kSpaVUnits;
-            ok = ptx::mbar_spin_warp(&v_full[slot], use & 1, abort_flag);
+            ok = ptx::mbar_spin(&v_full[slot], use & 1, abort_flag);
             if (!ok) break;
-            if (ptx::elect_one()) {
-              const uint32_t pl = (uint32_t)pd + (n & 1) * (kSpaPBuf / 16) + (u >> 1) * (kSpaPBlk / 16) + (u & 1) * 4;
-              const uint32_t vl = (uint32_t)vd + slot * (kSpaVUnit / 16);
+            const uint32_t pl = (uint32_t)pd + (n & 1) * (kSpaPBuf / 16) + (u >> 1) * (kSpaPBlk / 16) + (u & 1) * 4;
+            const uint32_t vl = (uint32_t)vd + slot * (kSpaVUnit / 16);
 #pragma unroll
-              for (int kk = 0; kk < 2; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                  ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (2048 / 16) + kk * (8192 / 16), v_hi,
-                                      a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
-              ptx::mma_commit_pair(&v_empty[slot]);
-              if (u == 3) ptx::mma_commit_pair(&p_empty[n & 1]);
-            }
-            __syncwarp();
+              for (int c = 0; c < 2; ++c)
+                ptx::mma_ss_pair_lo(tmem + kSpaTmO + c * 128, pl + kk * 2, p_hi, vl + c * (2048 / 16) + kk * (8192 / 16), v_hi,
+                                    a.idesc_pv, (t > first || u > 0 || kk > 0) ? 1u : 0u);
+            ptx::mma_commit_pair(&v_empty[slot]);
+            if (u == 3) ptx::mma_commit_pair(&p_empty[n & 1]);
           }
         }
       }
@@ -1242,7 +1255,9 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
       !make_tmap_gather4_16bit(&r1, p->key_rope, keys, 64, 128, 64, bf16) ||
       !spa_tmap(&vh, p->key, keys, std::min(box_keys, 32u), true, bf16) || !spa_tmap(&v8, p->key, keys, 8, true, bf16))
     return DSA_ERR_CUDA;
-  if (launch_after(spa_plan_kernel, dim3(1), dim3(kSpaPlanThreads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
+  // (barriers of 8 warps are cheaper than those of 32)
+  const int plan_threads = w.prefix_tiles + w.own_tiles <= 256 ? 256 : kSpaPlanThreads;
+  if (launch_after(spa_plan_kernel, dim3(1), dim3(plan_threads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
   if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k1, r1,
                    vh, v8, a) !=
       cudaSuccess)
