@@ -27,10 +27,22 @@ def require_cuda(*tensors):
             raise RuntimeError("dsa_triton_ascend_b200 runs on CUDA tensors only (there is no CPU path)")
 
 
-def same_device(first, *others):
+def one_device(first, *others):
+    """Refuse CPU tensors (RuntimeError, as require_cuda) and tensors of several devices; None is skipped."""
+    index = first.get_device()
+    if index < 0:
+        require_cuda(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            require_cuda(t)
             raise ValueError(f"tensors are on {first.device} and {t.device}: one device is needed")
+
+
+def int32_table(t, device):
+    """`t` as a contiguous int32 tensor on `device`: itself where it is one."""
+    if t.dtype == torch.int32 and t.is_contiguous() and t.device == device:
+        return t
+    return t.to(device=device, dtype=torch.int32).contiguous()
 
 
 @functools.lru_cache(maxsize=256)
@@ -54,7 +66,7 @@ def seq_tensor(lengths, device):
         return _cached_lengths(tuple(host), str(device)), host
     if isinstance(lengths, torch.Tensor):
         host = lengths.tolist() if not lengths.is_cuda else None
-        return lengths.to(device=device, dtype=torch.int32).contiguous(), host
+        return int32_table(lengths, device), host
     raise ValueError("actual_seq_lengths must be None, a list/tuple or an int32 tensor")
 
 

@@ -10,19 +10,36 @@ import ctypes
 import torch
 
 from . import _cabi
-from ._host import current_stream, device_guard, dtype_code, ptr, require_cuda, same_device, seq_tensor
+from ._host import current_stream, device_guard, dtype_code, int32_table, one_device, ptr, seq_tensor
 from .rotary import check_inv_freq, check_positions, section_sizes
 
 _VALID_D = (128, 256, 512)
 _D_ROPE = 64
+_PAIRS = (_D_ROPE // 2,)
+_STRUCT_SIZE = ctypes.sizeof(_cabi.DsaAppendParams)
 
 
 def _token_rows(t, step, align):
-    """`t` with a contiguous last dimension, strides that are multiples of `step` elements and a start on an `align`-byte
-    boundary: itself (a slice of a projection is read in place) or a copy."""
-    if t.stride(-1) != 1 or any(s % step for s in t.stride()[:-2]) or t.data_ptr() % align:
+    """(`t`, stride of a sequence, stride of a token) with a contiguous last dimension, strides that are multiples of `step`
+    elements and a start on an `align`-byte boundary: itself (a slice of a projection is read in place) or a copy."""
+    stride = t.stride()
+    sb, ss = stride[0], stride[-3]
+    if stride[-1] != 1 or sb % step or ss % step or t.data_ptr() % align:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        stride = t.stride()
+        sb, ss = stride[0], stride[-3]
+    return t, sb, ss
+
+
+def _check_pair(new, cache, tokens, blocks, block_size, width, dtype, what):
+    if new.shape != (*tokens, 1, width):
+        raise ValueError(f"{what} must have shape {(*tokens, 1, width)}, got {tuple(new.shape)}")
+    if cache.shape != (blocks, block_size, 1, width):
+        raise ValueError(f"the cache of {what} must have shape {(blocks, block_size, 1, width)}, got {tuple(cache.shape)}")
+    if new.dtype is not dtype or cache.dtype is not dtype:
+        raise ValueError("tokens and caches must share a dtype")
+    if not cache.is_contiguous():
+        raise ValueError("caches must be contiguous: they are updated in place")
 
 
 def latent_cache_append(
@@ -73,99 +90,76 @@ def latent_cache_append(
     """
     if layout not in ("BSND", "TND"):
         raise ValueError(f"layout must be BSND or TND, got {layout}")
-    lead = latent.ndim - 2
-    if latent.ndim != (4 if layout == "BSND" else 3) or latent.shape[-2] != 1:
-        raise ValueError(f"latent must be {'[B,S1,1,D]' if layout == 'BSND' else '[T1,1,D]'}, got {tuple(latent.shape)}")
-    if layout == "TND" and actual_seq_lengths_query is None:
+    tnd = layout == "TND"
+    if latent.ndim != (3 if tnd else 4) or latent.shape[-2] != 1:
+        raise ValueError(f"latent must be {'[T1,1,D]' if tnd else '[B,S1,1,D]'}, got {tuple(latent.shape)}")
+    if tnd and actual_seq_lengths_query is None:
         raise ValueError("TND tokens require cumulative actual_seq_lengths_query")
     if block_table is None or actual_seq_lengths_kv is None:
         raise ValueError("block_table and actual_seq_lengths_kv are required")
     if (index_key is None) != (index_cache is None):
         raise ValueError("index_key and index_cache go together")
-    D, tokens = latent.shape[-1], latent.shape[:lead]
+    D, tokens = latent.shape[-1], latent.shape[:-2]
     if D not in _VALID_D:
         raise ValueError(f"D must be one of {_VALID_D}, got {D}")
-    if latent_cache.ndim != 4:
+    if latent_cache.ndim != 4 or latent_cache.shape[1] < 1:
         raise ValueError("caches must be [block_num,block_size,1,D]")
     blocks, block_size = latent_cache.shape[0], latent_cache.shape[1]
-    d_index = index_key.shape[-1] if index_key is not None else 0
-    for new, cache, width, what in ((latent, latent_cache, D, "latent"), (key_rope, rope_cache, _D_ROPE, "key_rope"),
-                                    (index_key, index_cache, d_index, "index_key")):
-        if new is None:
-            continue
-        if tuple(new.shape) != (*tokens, 1, width):
-            raise ValueError(f"{what} must have shape {(*tokens, 1, width)}, got {tuple(new.shape)}")
-        if tuple(cache.shape) != (blocks, block_size, 1, width):
-            raise ValueError(f"the cache of {what} must have shape {(blocks, block_size, 1, width)}, got {tuple(cache.shape)}")
-        if new.dtype != latent.dtype or cache.dtype != latent.dtype:
-            raise ValueError("tokens and caches must share a dtype")
-        if not cache.is_contiguous():
-            raise ValueError("caches must be contiguous: they are updated in place")
-    if block_size < 1:
-        raise ValueError("block_size must be positive")
-    if index_key is not None and (d_index < 64 or d_index > 1024 or d_index % 2 or index_rotary_offset < 0 or
-                                  index_rotary_offset % 2 or index_rotary_offset + _D_ROPE > d_index):
-        raise ValueError(f"64 features from an even index_rotary_offset on must fit D_idx (even, 64 to 1024): got "
-                         f"{index_rotary_offset} and {d_index}")
-    inv_freq = check_inv_freq(inv_freq)
-    if inv_freq.numel() != _D_ROPE // 2:
-        raise ValueError(f"inv_freq must have {_D_ROPE // 2} entries, got {inv_freq.numel()}")
+    dtype = latent.dtype
     code = dtype_code(latent, (torch.bfloat16, torch.float16), "latent")
-    axes, sections = 1, (_D_ROPE // 2,)
+    _check_pair(latent, latent_cache, tokens, blocks, block_size, D, dtype, "latent")
+    _check_pair(key_rope, rope_cache, tokens, blocks, block_size, _D_ROPE, dtype, "key_rope")
+    d_index = 0
+    if index_key is not None:
+        d_index = index_key.shape[-1]
+        _check_pair(index_key, index_cache, tokens, blocks, block_size, d_index, dtype, "index_key")
+        if (d_index < 64 or d_index > 1024 or d_index % 2 or index_rotary_offset < 0 or index_rotary_offset % 2 or
+                index_rotary_offset + _D_ROPE > d_index):
+            raise ValueError(f"64 features from an even index_rotary_offset on must fit D_idx (even, 64 to 1024): got "
+                             f"{index_rotary_offset} and {d_index}")
+    inv_freq = check_inv_freq(inv_freq)
+    if inv_freq.shape[0] != _D_ROPE // 2:
+        raise ValueError(f"inv_freq must have {_D_ROPE // 2} entries, got {inv_freq.shape[0]}")
+    axes, sections = 1, _PAIRS
     if positions is not None:
         axes, sections = section_sizes(axis_sections, _D_ROPE // 2)
         positions = check_positions(positions, tokens, axis_sections)
     elif axis_sections is not None:
         raise ValueError("axis_sections needs positions")
+    code_w = code
     if norm_weight is not None:
-        if tuple(norm_weight.shape) != (D,) or norm_weight.dtype not in (latent.dtype, torch.float32):
+        if norm_weight.shape != (D,) or (norm_weight.dtype is not dtype and norm_weight.dtype is not torch.float32):
             raise ValueError(f"norm_weight must be [{D}] in the latents' dtype or float32")
         norm_weight = norm_weight.contiguous()
         if norm_weight.data_ptr() % 16:
             norm_weight = norm_weight.clone()
-    require_cuda(latent, key_rope, latent_cache, rope_cache, inv_freq, block_table, index_key, index_cache, positions,
-                 norm_weight)
-    same_device(latent, key_rope, latent_cache, rope_cache, inv_freq, index_key, index_cache, positions, norm_weight)
+        if norm_weight.dtype is torch.float32:
+            code_w = _cabi.DTYPE_FP32
+    one_device(latent, key_rope, latent_cache, rope_cache, inv_freq, index_key, index_cache, positions, norm_weight)
     dev = latent.device
-    if latent_cache.data_ptr() % 16 or any(c is not None and c.data_ptr() % 4 for c in (rope_cache, index_cache)):
+    if latent_cache.data_ptr() % 16 or rope_cache.data_ptr() % 4 or (index_cache is not None and index_cache.data_ptr() % 4):
         raise ValueError("caches must start on 16-byte boundaries (latents) and 4-byte boundaries (the others)")
     seq_q, _ = seq_tensor(actual_seq_lengths_query, dev)
     seq_k, _ = seq_tensor(actual_seq_lengths_kv, dev)
-    block_table = block_table.to(device=dev, dtype=torch.int32).contiguous()
-    batch = seq_q.shape[0] if layout == "TND" else latent.shape[0]
-    if block_table.ndim != 2 or block_table.shape[0] != batch or tuple(seq_k.shape) != (batch,) or (
-            seq_q is not None and tuple(seq_q.shape) != (batch,)):
+    block_table = int32_table(block_table, dev)
+    batch = seq_q.shape[0] if tnd else tokens[0]
+    if block_table.ndim != 2 or block_table.shape[0] != batch or seq_k.shape != (batch,) or (
+            seq_q is not None and seq_q.shape != (batch,)):
         raise ValueError(f"block_table and lengths must have an entry for each of the {batch} sequences")
-    if latent.numel() == 0 or batch == 0 or latent_cache.numel() == 0 or block_table.shape[1] == 0:
+    if latent.numel() == 0 or batch == 0 or blocks == 0 or block_table.shape[1] == 0:
         return latent_cache, rope_cache, index_cache
-    latent, key_rope = _token_rows(latent, 8, 16), _token_rows(key_rope, 2, 4)
+    latent, latent_b, latent_s = _token_rows(latent, 8, 16)
+    key_rope, rope_b, rope_s = _token_rows(key_rope, 2, 4)
+    index_b = index_s = 0
     if index_key is not None:
-        index_key = _token_rows(index_key, 2, 4)
+        index_key, index_b, index_s = _token_rows(index_key, 2, 4)
 
-    p = _cabi.DsaAppendParams()
-    p.struct_size = ctypes.sizeof(_cabi.DsaAppendParams)
-    p.dtype = code
-    p.latent, p.key_rope, p.index_key, p.norm_weight = ptr(latent), ptr(key_rope), ptr(index_key), ptr(norm_weight)
-    p.positions, p.inv_freq = ptr(positions), ptr(inv_freq)
-    p.seq_q, p.seq_k, p.block_table = ptr(seq_q), ptr(seq_k), ptr(block_table)
-    p.latent_cache, p.rope_cache, p.index_cache = ptr(latent_cache), ptr(rope_cache), ptr(index_cache)
-    p.latent_stride_b, p.latent_stride_s = latent.stride(0), latent.stride(lead - 1)
-    p.rope_stride_b, p.rope_stride_s = key_rope.stride(0), key_rope.stride(lead - 1)
-    if index_key is not None:
-        p.index_stride_b, p.index_stride_s = index_key.stride(0), index_key.stride(lead - 1)
-        p.d_index, p.index_offset = d_index, index_rotary_offset
-        p.index_interleaved = 1 if index_interleaved else 0
-    p.layout_q, p.batch, p.s1 = _cabi.LAYOUTS[layout], batch, latent.shape[lead - 1]
-    p.d, p.d_rope = D, _D_ROPE
-    p.block_size, p.max_blocks = block_size, block_table.shape[1]
-    p.interleaved = 1 if interleaved else 0
-    p.positions_64bit = 1 if positions is not None and positions.dtype == torch.int64 else 0
-    p.dtype_w = _cabi.DTYPE_FP32 if norm_weight is not None and norm_weight.dtype == torch.float32 else code
-    p.axes = axes
-    for i, n in enumerate(sections):
-        p.sections[i] = n
-    p.norm_eps = float(norm_eps)
-    p.key_rows = blocks * block_size
+    p = _cabi.DsaAppendParams(
+        _STRUCT_SIZE, code, latent.data_ptr(), key_rope.data_ptr(), ptr(index_key), ptr(norm_weight), ptr(positions),
+        inv_freq.data_ptr(), ptr(seq_q), seq_k.data_ptr(), block_table.data_ptr(), latent_cache.data_ptr(), rope_cache.data_ptr(),
+        ptr(index_cache), latent_b, latent_s, rope_b, rope_s, index_b, index_s, _cabi.LAYOUTS[layout], batch, tokens[-1], D,
+        _D_ROPE, d_index, index_rotary_offset, block_size, block_table.shape[1], bool(interleaved), bool(index_interleaved),
+        positions is not None and positions.dtype is torch.int64, code_w, axes, sections, norm_eps, blocks * block_size)
     with device_guard(dev):
         _cabi.check(_cabi.lib.dsa_latent_append(ctypes.byref(p), current_stream(dev)), "latent_cache_append")
     return latent_cache, rope_cache, index_cache

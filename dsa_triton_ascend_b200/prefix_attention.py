@@ -8,10 +8,11 @@ import ctypes
 import torch
 
 from . import _cabi
-from ._host import (current_stream, device_guard, dtype_code, note_launch, packed, ptr, require_cuda, same_device,
-                    seq_tensor, workspace)
+from ._host import (current_stream, device_guard, dtype_code, int32_table, note_launch, one_device, packed, ptr, seq_tensor,
+                    workspace)
 
 _D, _D_ROPE = 512, 64
+_STRUCT_SIZE = ctypes.sizeof(_cabi.DsaSpaParams)
 _kernel = _cabi.KERNEL_AUTO
 
 
@@ -70,20 +71,22 @@ def shared_prefix_attention(
         raise ValueError(f"query must be {'[T1,N1,D]' if tnd else '[B,S1,N1,D]'}, got {tuple(query.shape)}")
     if tnd and actual_seq_lengths_query is None:
         raise ValueError("TND query requires cumulative actual_seq_lengths_query")
-    N1, D = query.shape[-2:]
+    lead, N1, D = query.shape[:-2], query.shape[-2], query.shape[-1]
     if D != _D:
         raise ValueError(f"D must be {_D}, got {D}")
     if N1 < 1:
         raise ValueError(f"N1 must be positive, got {N1}")
-    if tuple(query_rope.shape) != (*query.shape[:-1], _D_ROPE):
-        raise ValueError(f"query_rope must have shape {(*query.shape[:-1], _D_ROPE)}, got {tuple(query_rope.shape)}")
-    if key.ndim != 4 or key.shape[2] != 1 or key.shape[3] != D or key.shape[0] < 1 or key.shape[1] < 1:
+    if query_rope.shape != (*lead, N1, _D_ROPE):
+        raise ValueError(f"query_rope must have shape {(*lead, N1, _D_ROPE)}, got {tuple(query_rope.shape)}")
+    blocks, page = key.shape[0], key.shape[1]
+    if key.shape != (blocks, page, 1, D) or blocks < 1 or page < 1:
         raise ValueError(f"key must be [block_num,block_size,1,{D}] with a block at least, got {tuple(key.shape)}")
-    if tuple(key_rope.shape) != (*key.shape[:3], _D_ROPE):
-        raise ValueError(f"key_rope must have shape {(*key.shape[:3], _D_ROPE)}, got {tuple(key_rope.shape)}")
-    if (block_size or key.shape[1]) != key.shape[1]:
+    if key_rope.shape != (blocks, page, 1, _D_ROPE):
+        raise ValueError(f"key_rope must have shape {(blocks, page, 1, _D_ROPE)}, got {tuple(key_rope.shape)}")
+    if block_size and block_size != page:
         raise ValueError("block_size must equal the cache's block dimension")
-    if not (query.dtype == key.dtype == query_rope.dtype == key_rope.dtype):
+    dtype = query.dtype
+    if key.dtype is not dtype or query_rope.dtype is not dtype or key_rope.dtype is not dtype:
         raise ValueError("query, key, query_rope and key_rope must share a dtype")
     code = dtype_code(query, (torch.bfloat16, torch.float16), "query")
     prefix, prefix_t = shared_prefix_length, None
@@ -94,46 +97,37 @@ def shared_prefix_attention(
     prefix = min(int(prefix), 2**31 - 1)
     if prefix < 0:
         raise ValueError(f"shared_prefix_length must not be negative, got {prefix}")
-    require_cuda(query, key, query_rope, key_rope, block_table, prefix_t)
-    same_device(query, key, query_rope, key_rope, block_table, prefix_t)
+    one_device(query, key, query_rope, key_rope, prefix_t)
     dev = query.device
     seq_q, _ = seq_tensor(actual_seq_lengths_query, dev)
     seq_k, _ = seq_tensor(actual_seq_lengths_kv, dev)
-    B = seq_q.shape[0] if tnd else query.shape[0]
-    block_table = block_table.to(dtype=torch.int32).contiguous()
-    if block_table.ndim != 2 or block_table.shape[0] != B or tuple(seq_k.shape) != (B,) or (
-            seq_q is not None and tuple(seq_q.shape) != (B,)):
+    B = seq_q.shape[0] if tnd else lead[0]
+    block_table = int32_table(block_table, dev)
+    if block_table.ndim != 2 or block_table.shape[0] != B or seq_k.shape != (B,) or (
+            seq_q is not None and seq_q.shape != (B,)):
         raise ValueError(f"block_table and lengths must have an entry for each of the {B} sequences")
     query, query_rope, key, key_rope = packed(query), packed(query_rope), packed(key), packed(key_rope)
-    s1 = query.shape[0] if tnd else query.shape[1]
+    s1 = lead[-1]
 
     out = torch.empty_like(query)
     stat_shape = (1, s1, N1) if tnd else (B, 1, s1, N1)
     sm_max = torch.empty(stat_shape, dtype=torch.float32, device=dev)
-    sm_sum = torch.empty(stat_shape, dtype=torch.float32, device=dev)
+    sm_sum = torch.empty_like(sm_max)
     if out.numel() == 0:
         return out, sm_max, sm_sum
     if B == 0:      # tokens that belong to no sequence
         return out.zero_(), sm_max.zero_(), sm_sum.zero_()
 
-    p = _cabi.DsaSpaParams()
-    p.struct_size = ctypes.sizeof(_cabi.DsaSpaParams)
-    p.kernel = _kernel
-    p.query, p.query_rope, p.key, p.key_rope = ptr(query), ptr(query_rope), ptr(key), ptr(key_rope)
-    p.seq_q, p.seq_k, p.block_table, p.prefix_device = ptr(seq_q), ptr(seq_k), ptr(block_table), ptr(prefix_t)
-    p.out, p.softmax_max, p.softmax_sum = ptr(out), ptr(sm_max), ptr(sm_sum)
-    p.layout_q, p.dtype = _cabi.LAYOUTS[layout_query], code
-    p.batch, p.s1, p.n1, p.d, p.d_rope = B, s1, N1, D, _D_ROPE
-    p.block_size, p.max_blocks = key.shape[1], block_table.shape[1]
-    p.prefix, p.sparse_mode = prefix, sparse_mode
-    p.return_lse = 1 if return_softmax_lse else 0
-    p.scale = float(scale_value)
-    p.key_rows = key.shape[0] * key.shape[1]
+    p = _cabi.DsaSpaParams(
+        _STRUCT_SIZE, _kernel, query.data_ptr(), query_rope.data_ptr(), key.data_ptr(), key_rope.data_ptr(), ptr(seq_q),
+        seq_k.data_ptr(), block_table.data_ptr(), ptr(prefix_t), out.data_ptr(), sm_max.data_ptr(), sm_sum.data_ptr(),
+        _cabi.LAYOUTS[layout_query], code, B, s1, N1, D, _D_ROPE, page, block_table.shape[1], prefix, sparse_mode,
+        bool(return_softmax_lse), scale_value, blocks * page)
     with device_guard(dev):
         nbytes = ctypes.c_size_t(0)
         _cabi.check(_cabi.lib.dsa_spa_workspace_bytes(ctypes.byref(p), ctypes.byref(nbytes)), "shared_prefix_attention")
         ws = workspace(nbytes.value, dev)
-        _cabi.check(_cabi.lib.dsa_spa_forward(ctypes.byref(p), ws.data_ptr(), ws.numel(), current_stream(dev)),
+        _cabi.check(_cabi.lib.dsa_spa_forward(ctypes.byref(p), ws.data_ptr(), nbytes.value, current_stream(dev)),
                     "shared_prefix_attention")
         note_launch("shared_prefix_attention", ws, dev)
     return out, sm_max, sm_sum

@@ -8,9 +8,10 @@ import ctypes
 import torch
 
 from . import _cabi
-from ._host import current_stream, device_guard, dtype_code, ptr, require_cuda, same_device
+from ._host import current_stream, device_guard, dtype_code, one_device
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_STRUCT_SIZE = ctypes.sizeof(_cabi.DsaRopeParams)
 MAX_AXES = 4
 
 
@@ -26,10 +27,10 @@ def section_sizes(axis_sections, pairs):
 
 def check_positions(positions, tokens, axis_sections, what="positions"):
     """`positions` of shape `tokens`, or [axes, *tokens] where axis_sections are given, as a contiguous tensor."""
-    want = tuple(tokens) if axis_sections is None else (len(axis_sections), *tokens)
-    if positions.dtype not in (torch.int32, torch.int64):
+    want = tokens if axis_sections is None else (len(axis_sections), *tokens)
+    if positions.dtype is not torch.int32 and positions.dtype is not torch.int64:
         raise ValueError(f"{what} must be int32 or int64, got {positions.dtype}")
-    if tuple(positions.shape) != want:
+    if positions.shape != want:
         raise ValueError(f"{what} must have shape {want}, got {tuple(positions.shape)}")
     return positions.contiguous()
 
@@ -41,36 +42,36 @@ def check_inv_freq(inv_freq):
 
 
 def _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what):
-    if layout not in ("BSND", "TND"):
+    if layout == "BSND":
+        if x.ndim != 4:
+            raise ValueError(f"{what} must be [B,S,N,D], got {tuple(x.shape)}")
+        batch, s1, n, D = x.shape
+        stride_b, stride_s, stride_n, stride_d = x.stride()
+        tokens = (batch, s1)
+    elif layout == "TND":
+        if x.ndim != 3:
+            raise ValueError(f"{what} must be [T,N,D], got {tuple(x.shape)}")
+        s1, n, D = x.shape
+        stride_s, stride_n, stride_d = x.stride()
+        batch, stride_b, tokens = 1, 0, (s1,)
+    else:
         raise ValueError(f"layout must be BSND or TND, got {layout}")
-    if x.ndim != (4 if layout == "BSND" else 3):
-        raise ValueError(f"{what} must be {'[B,S,N,D]' if layout == 'BSND' else '[T,N,D]'}, got {tuple(x.shape)}")
     code = dtype_code(x, _DTYPES, what)
     inv_freq = check_inv_freq(inv_freq)
-    pairs, D = inv_freq.numel(), x.shape[-1]
+    pairs = inv_freq.shape[0]
     if D > 1024 or rotary_offset < 0 or rotary_offset + 2 * pairs > D:
         raise ValueError(f"{pairs} pairs from feature {rotary_offset} on do not fit {D} features (at most 1024)")
     axes, sections = section_sizes(axis_sections, pairs)
-    positions = check_positions(positions, x.shape[:-2], axis_sections)
-    require_cuda(x, positions, inv_freq)
-    same_device(x, positions, inv_freq)
-    if x.stride(-1) != 1 and D > 1:
-        x = x.contiguous()
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out.numel() == 0:
+    positions = check_positions(positions, tokens, axis_sections)
+    one_device(x, positions, inv_freq)
+    if stride_d != 1:
+        return _rotate(x.contiguous(), positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if batch == 0 or s1 == 0 or n == 0:
         return out
-    p = _cabi.DsaRopeParams()
-    p.struct_size = ctypes.sizeof(_cabi.DsaRopeParams)
-    p.inverse = 1 if inverse else 0
-    p.x, p.positions, p.inv_freq, p.out = ptr(x), ptr(positions), ptr(inv_freq), ptr(out)
-    p.stride_b = x.stride(0) if layout == "BSND" else 0
-    p.stride_s, p.stride_n = x.stride(-3), x.stride(-2)
-    p.dtype, p.positions_64bit = code, 1 if positions.dtype == torch.int64 else 0
-    p.batch, p.s1 = (x.shape[0], x.shape[1]) if layout == "BSND" else (1, x.shape[0])
-    p.n, p.d = x.shape[-2], D
-    p.pairs, p.offset, p.interleaved, p.axes = pairs, rotary_offset, 1 if interleaved else 0, axes
-    for i, n in enumerate(sections):
-        p.sections[i] = n
+    p = _cabi.DsaRopeParams(
+        _STRUCT_SIZE, inverse, x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), out.data_ptr(), stride_b, stride_s,
+        stride_n, code, positions.dtype is torch.int64, batch, s1, n, D, pairs, rotary_offset, bool(interleaved), axes, sections)
     dev = x.device
     with device_guard(dev):
         _cabi.check(_cabi.lib.dsa_rope(ctypes.byref(p), current_stream(dev)), "rotary_embedding")
