@@ -3,8 +3,8 @@
 //
 // Rows.  A row is a (token, head) pair; rows are flat in memory (token * n1 + head), so that 128 consecutive ones are one
 // M = 128 tile whatever the number of heads.  A job is a row tile against a range of key positions:
-//   - a sequence of few rows (up to 64) that sees the whole prefix is PACKED: its rows meet the prefix together with those
-//     of its neighbours, in tiles cut from the flat rows of the whole batch (prefix jobs), and its own keys in a job of its own;
+//   - where it pays, a sequence of few rows (up to 64) that sees the whole prefix is PACKED: its rows meet the prefix together
+//     with those of its neighbours, in tiles cut from the flat rows of the whole batch (prefix jobs), and its own keys in a job of its own;
 //   - every other sequence is cut into row tiles of its own, each over all the tile's visible keys.  Its tiles are full (or
 //     nearly), so that packing would save nothing; that the prefix is the same pages for everybody then shows as L2 hits.
 // A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into equal
@@ -55,7 +55,12 @@ constexpr int kSpaKeys = 128;        // keys per tile
 constexpr int kSpaThreads = 512;
 constexpr int kSpaQkWarp0 = 3, kSpaSoftWarp0 = 4, kSpaPvWarp = 12, kSpaQkWarp1 = 13, kSpaKWarp1 = 14, kSpaVWarp1 = 15;
 constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
-constexpr int kSpaPackKeys = 256;    // a shorter prefix is not worth the partials
+constexpr int kSpaPackKeys = 128;    // prefix that can save a tile
+// Packing pays when the key tiles that it saves outweigh the partials that it makes, 40 tiles and one per 8 rows.  us a call
+// packed / not: 64 x 64 heads behind 512 keys 46.5 / 39 (saves 128 tiles), 8192 115 / 140 (2048); 32 x 64 heads behind 4096
+// 49 / 55 (512); 64 x 16 heads behind 256 28.5 / 27 (112), 512 28.5 / 31.5 (224), 1024 31.5 / 39.6 (448); 64 x 32 heads
+// behind 4096 53 / 87; 8 x 16 heads behind 512 19.6 / 18.5 (28).
+__host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 40 + rows / 8; }
 constexpr int kSpaPlanThreads = 1024;
 constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
 constexpr int kSpaSnapTiles = 3;     // tiles that a share may be longer by so that it ends with its job
@@ -206,6 +211,30 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     ref = 0x7FFFFFFF - (int32_t)(uint32_t)best;
     prefix = max(0, min(asked, (int32_t)(best >> 32)));
+    // worth it?  (prefix = 0: nothing is packed)
+    int32_t n = 0, r = 0;
+    for (int32_t b = tid; b < p.seq.batch; b += nt) {
+      const SpaSeq s = spa_seq(p, b, prefix);
+      if (s.packed) { ++n; r += s.act_q * p.n1; }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+      r += __shfl_xor_sync(0xffffffffu, r, o);
+    }
+    if (lane == 0) { sum_s[0][warp] = n; sum_s[1][warp] = r; }
+    __syncthreads();
+    n = lane < warps ? sum_s[0][lane] : 0;
+    r = lane < warps ? sum_s[1][lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+      r += __shfl_xor_sync(0xffffffffu, r, o);
+    }
+    const int64_t saved = (int64_t)n * (prefix / kSpaKeys) -
+                          (int64_t)((r + kSpaRows - 1) / kSpaRows) * ((prefix + kSpaKeys - 1) / kSpaKeys);
+    if (saved < spa_pack_least(r)) prefix = 0;
+    __syncthreads();                          // (sum_s is written again)
   }
 
   const int32_t places = p.prefix_tiles + p.own_tiles, rows = p.rows * p.n1;

@@ -275,6 +275,75 @@ def test_many_sequences_and_long_ones(kind):
     verify(make(11, "BSND", [1] * 2, [20000, 9000], 8, 128, 8999), kind)
 
 
+@pytest.mark.parametrize("page", [1, 8, 16, 24, 32, 48, 64, 100, 128])
+@pytest.mark.parametrize("prefix", [500, 768])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_packed_rows_over_pages(page, prefix, dtype):
+    """Enough sequences of few rows that they meet the prefix together, in tiles that mix sequences."""
+    lens = [prefix + 1 + (13 * i) % 300 for i in range(64)]
+    verify(make(page, "BSND", [1] * 64, lens, 4, page, prefix, dtype), "tensor")
+
+
+@pytest.mark.parametrize("prefix", [255, 256, 257, 383, 384, 1000, 1024, 2049])
+@pytest.mark.parametrize("heads,batch", [(3, 61), (64, 70), (20, 90)])
+def test_packed_rows_behind_prefixes(prefix, heads, batch):
+    lens = [prefix + (7 * i) % 200 for i in range(batch)]       # (some hold nothing but the prefix)
+    verify(make(prefix, "BSND", [1] * batch, lens, heads, 64, prefix), "tensor")
+
+
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
+@pytest.mark.parametrize("mode", [0, 3])
+def test_packed_rows_beside_others(layout, mode):
+    """Sequences of one to three tokens, of none, of a whole chunk, shorter than the prefix, without keys: packed ones between them."""
+    q_lens = [1 + i % 3 for i in range(80)]
+    kv = [900 + (11 * i) % 333 for i in range(80)]
+    q_lens[5], q_lens[17], kv[9], kv[21], kv[40] = 0, 3 if layout == "BSND" else 40, 512, 3, 0
+    verify(make(31, layout, q_lens, kv, 8, 64, 896, s1=4 if layout == "BSND" else None, tail=5 if layout == "TND" else 0),
+           "tensor", mode=mode)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_in_masked_places_of_packed_rows(bad):
+    q_lens, kv = [2] * 70, [700 + i for i in range(70)]
+    s = make(32, "BSND", q_lens, kv, 8, 16, 640)
+    for b in (0, 33, 69):
+        row = rows_of(s["table"], b, torch.tensor([kv[b] - 1], device="cuda"), 16, s["cache"].shape[0])
+        s["cache"].view(-1, 512)[row, 77] = bad
+    flat = lambda t: t.reshape(-1, *t.shape[-2:])
+    want, room = reference(flat(s["q"]), flat(s["qr"]), s["cache"], s["rope"], s["table"], q_lens, kv, s["starts"], 1 / 24, 3)
+    got = [g.reshape(w.shape) for g, w in zip(call(s), want)]
+    sees = torch.zeros(140, dtype=torch.bool, device="cuda")
+    sees[[1, 67, 139]] = True
+    check([g[~sees] for g in got], [w[~sees] for w in want], [r[~sees] for r in room])
+    assert not torch.isfinite(got[0][sees][..., 77]).any()
+
+
+def test_absent_blocks_of_packed_rows():
+    s = make(33, "BSND", [1] * 70, [700 + i for i in range(70)], 8, 64, 640)
+    s["table"][:, 3] = -1
+    s["table"][7, 10] = s["cache"].shape[0]
+    verify(s, "tensor")
+
+
+def test_packed_scores_that_outgrow_the_first_tile():
+    s = make(34, "BSND", [1] * 70, [1300 + i for i in range(70)], 8, 64, 1280)
+    u = torch.nn.functional.normalize(torch.randn(512, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"), dim=0)
+    s["q"] = (s["q"].float() * 0.3 + 20 * u).to(s["q"].dtype)
+    row = rows_of(s["table"], 0, torch.arange(1280, device="cuda"), 64, s["cache"].shape[0])
+    c = s["cache"].view(-1, 512)
+    c[row] = (c[row].float() * 0.5 + torch.linspace(0, 8, 1280, device="cuda")[:, None] * u).to(c.dtype)
+    verify(s, "tensor", scale=1.0)
+
+
+def test_the_longest_sequence_lends_the_prefix():
+    """The pages of the others hold other numbers where the prefix would be: what counts is the first of the longest ones'."""
+    s = make(35, "BSND", [1] * 70, [700] * 30 + [900] + [701] * 39, 8, 64, 640)
+    got = call(s)
+    s["table"][:30, :10] = s["table"][30, 10]
+    s["table"][31:, :10] = -1
+    assert all(torch.equal(a, b) for a, b in zip(call(s), got))
+
+
 def test_single_tokens_of_many_small_sequences():
     """130 sequences of one head: a row tile holds rows of 128 sequences."""
     lens = [257 + i for i in range(130)]
