@@ -593,7 +593,7 @@ __device__ __forceinline__ void spa_v_boxes(const SpaArgs& a, const SpaLoads& o)
 }
 
 // Pages that are no multiple of 8: rows are gathered, four a load.  Lane i holds the positions 4 i .. 4 i + 3 of the CTA's 64 (K) or
-// of the tile's 128 (V); one lane issues (lanes that each issue their own cost 130 cycles a load).
+// of the tile's 128 (V); one elected lane issues.
 template <bool kV>
 __device__ __forceinline__ void spa_gather(const SpaArgs& a, const SpaLoads& o) {
   const int lane = threadIdx.x & 31;
@@ -627,19 +627,21 @@ __device__ __forceinline__ void spa_gather(const SpaArgs& a, const SpaLoads& o) 
         const int l = kV ? u * 8 + q : q;
         const int32_t x0 = __shfl_sync(0xffffffffu, r[0], l), x1 = __shfl_sync(0xffffffffu, r[1], l),
                       x2 = __shfl_sync(0xffffffffu, r[2], l), x3 = __shfl_sync(0xffffffffu, r[3], l);
-        if (lane != 0) continue;
-        if (kV) {
+        if (ptx::elect_one()) {
+          if (kV) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            ptx::tma_gather4_2d_pair(dst + (q >> 1) * 4096 + c * 1024 + (q & 1) * 512, o.gather, bar,
-                                     (c >> 1) * 256 + o.rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
-        } else if (u < 4) {
+            for (int c = 0; c < 4; ++c)
+              ptx::tma_gather4_2d_pair(dst + (q >> 1) * 4096 + c * 1024 + (q & 1) * 512, o.gather, bar,
+                                       (c >> 1) * 256 + o.rank * 128 + (c & 1) * 64, x0, x1, x2, x3);
+          } else if (u < 4) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            ptx::tma_gather4_2d_pair(dst + (q >> 1) * 2048 + e * 1024 + (q & 1) * 512, o.gather, bar, u * 128 + e * 64, x0, x1, x2, x3);
-        } else {
-          ptx::tma_gather4_2d_pair(dst + q * 512, o.rope_gather, bar, 0, x0, x1, x2, x3);
+            for (int e = 0; e < 2; ++e)
+              ptx::tma_gather4_2d_pair(dst + (q >> 1) * 2048 + e * 1024 + (q & 1) * 512, o.gather, bar, u * 128 + e * 64, x0, x1, x2, x3);
+          } else {
+            ptx::tma_gather4_2d_pair(dst + q * 512, o.rope_gather, bar, 0, x0, x1, x2, x3);
+          }
         }
+        __syncwarp();
       }
       __syncwarp();
     }
