@@ -761,7 +761,7 @@ using namespace dsa;
 
 extern "C" {
 
-int dsa_abi_version(void) { return 7; }
+int dsa_abi_version(void) { return 8; }
 
 unsigned long long dsa_kernel_launch_count(void) { return launch_counter().load(std::memory_order_relaxed); }
 

@@ -265,8 +265,10 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
     }
     if (p.return_lse && tid < kSfaSimtHeads && h0 + tid < p.n1) {
       const float lt = l_s[tid];
-      p.softmax_max[(int64_t)row * p.n1 + h0 + tid] = lt > 0.f ? m_s[tid] : 0.f;
-      p.softmax_sum[(int64_t)row * p.n1 + h0 + tid] = lt > 0.f ? lt : 0.f;
+      // (dense: a row whose sum is not a number says so)
+      const bool nan = kDense && lt != lt;
+      p.softmax_max[(int64_t)row * p.n1 + h0 + tid] = nan ? lt : lt > 0.f ? m_s[tid] : 0.f;
+      p.softmax_sum[(int64_t)row * p.n1 + h0 + tid] = nan ? lt : lt > 0.f ? lt : 0.f;
     }
   }
 }

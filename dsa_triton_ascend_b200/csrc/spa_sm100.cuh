@@ -622,7 +622,7 @@ __device__ __forceinline__ void spa_gather(const SpaArgs& a, const SpaLoads& o) 
       if (o.rank == 0 && lane == 0)
         ptx::mbar_arrive_expect_tx(&o.full[slot], kV ? 2 * kSpaVUnit : u < 4 ? 2 * kSpaKUnit : kSpaKUnit);
       const uint32_t dst = o.dst + slot * (kV ? kSpaVUnit : kSpaKUnit), bar = o.full_lead + slot * 8;
-#pragma unroll 1
+#pragma unroll 4
       for (int q = 0; q < (kV ? 8 : 16); ++q) {
         const int l = kV ? u * 8 + q : q;
         const int32_t x0 = __shfl_sync(0xffffffffu, r[0], l), x1 = __shfl_sync(0xffffffffu, r[1], l),
@@ -1025,7 +1025,8 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         }
         if (g == 0 && half == 0 && trow < j.nrows && a.p.softmax_max != nullptr) {
           const bool give = a.p.return_lse && any;
-          a.p.softmax_max[(int64_t)j.row0 + trow] = give ? m_true * 0.6931471805599453f : 0.f;
+          // (a row whose sum is not a number has no maximum either)
+          a.p.softmax_max[(int64_t)j.row0 + trow] = give ? (total == total ? m_true * 0.6931471805599453f : total) : 0.f;
           a.p.softmax_sum[(int64_t)j.row0 + trow] = give ? total : 0.f;
         }
       }
@@ -1157,7 +1158,7 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
     ptx::st_global_v8((unsigned char*)p.out + (int64_t)row * 1024 + cols * 2, out);
     if (cols == 0 && p.softmax_max != nullptr) {
       const bool give = p.return_lse && any;
-      p.softmax_max[row] = give ? mx * 0.6931471805599453f : 0.f;
+      p.softmax_max[row] = give ? (den == den ? mx * 0.6931471805599453f : den) : 0.f;
       p.softmax_sum[row] = give ? den : 0.f;
     }
   }

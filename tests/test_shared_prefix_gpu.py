@@ -402,6 +402,62 @@ def test_the_prefix_length_can_live_on_the_device():
         check(held, want, room, str(p))
 
 
+@pytest.mark.parametrize("kind", KERNELS)
+def test_tables_without_columns_and_batches_without_keys(kind):
+    s = make(40, "BSND", [2] * 3, [50, 60, 70], 16, 16, 48)
+    for t in (dict(s, table=s["table"][:, :0]), dict(s, kv_lens=[0, 0, 0]), dict(s, kv_lens=[-3, 0, -1]), dict(s, seq_q=[0, 0, 0])):
+        with kernel(kind):
+            got = call(t)
+        assert not any(g.any() for g in got)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+def test_lengths_past_the_table(kind):
+    """Positions behind the table's last block do not exist."""
+    s = make(41, "BSND", [1] * 3, [300, 200, 320], 16, 16, 0)
+    s["table"] = s["table"][:, :20].contiguous()
+    lens = [2**31 - 1, 200, 5000]
+    want, room = reference(s["q"][:, 0], s["qr"][:, 0], s["cache"], s["rope"],
+                           torch.where(s["table"] >= 0, s["table"], torch.full_like(s["table"], 10**6)), [1] * 3, [320, 200, 320],
+                           [0, 1, 2], 1 / 24, 3)
+    s["table"][0, 19] = s["table"][1, 13:] = -1        # (blocks that were never filled: absent)
+    with kernel(kind):
+        got = call(dict(s, kv_lens=lens))
+    got = [g.reshape(w.shape) for g, w in zip(got, want)]
+    check([g[2:] for g in got], [w[2:] for w in want], [r[2:] for r in room], kind)
+    # sequence 0 claims positions 300 .. 303 of its 19th block, which no token filled: they hold NaN and are visible
+    assert torch.isnan(got[0][0]).all() and torch.isfinite(got[0][1:]).all()
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("heads", [16, 128])
+def test_a_query_that_is_not_a_number_spoils_its_own_row_only(kind, heads):
+    s = make(42, "BSND", [2] * 3, [300, 290, 310], heads, 64, 256)
+    flat = lambda t: t.reshape(-1, *t.shape[-2:])
+    want, room = reference(flat(s["q"]), flat(s["qr"]), s["cache"], s["rope"], s["table"], s["q_lens"], s["kv_lens"],
+                           s["starts"], 1 / 24, 3)
+    s["q"][1, 0, 3, 100] = float("nan")
+    with kernel(kind):
+        got = [g.reshape(w.shape).clone() for g, w in zip(call(s), want)]
+    assert all(torch.isnan(g[2, 3]).all() for g in got)
+    for g, w in zip(got, want):
+        g[2, 3] = w[2, 3].to(g.dtype)
+    check(got, want, room, kind)
+
+
+@pytest.mark.parametrize("heads,batch", [(256, 3), (300, 2), (16, 700), (1, 1500)])
+def test_many_heads_and_many_sequences(heads, batch):
+    lens = [130 + (i * 7) % 150 for i in range(batch)]
+    verify(make(43, "BSND", [1] * batch, lens, heads, 64, 128), "tensor")
+
+
+@pytest.mark.parametrize("heads", [16, 128])
+def test_a_prompt_of_its_own(heads):
+    """One long sequence, every token a query: a causal prefill over the cache."""
+    verify(make(44, "TND", [700], [700], heads, 64, 0), "tensor")
+    verify(make(45, "TND", [300, 5, 200], [1100, 5, 700], heads, 32, 0), "tensor")
+
+
 def test_calls_on_two_streams_at_once():
     a = make(17, "BSND", [1] * 8, [2000 + 64 * i for i in range(8)], 16, 64, 1920)
     b = make(18, "BSND", [1] * 30, [900 + 64 * i for i in range(30)], 64, 64, 832, "fp16")
