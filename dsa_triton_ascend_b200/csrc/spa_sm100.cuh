@@ -96,7 +96,7 @@ struct SpaJob {
   int32_t tile0, tiles;     // first tile in the order of all jobs' tiles, and their number
   int32_t vis0;             // positions that the first row's token sees (mode 3: one more per token)
   int32_t head0;            // head of the first row
-  int32_t packed;           // 1: rows of packed sequences against the prefix; the rows of other sequences are skipped
+  int32_t packed;           // 1: rows of packed sequences against the prefix (those of other sequences are not read)
   int32_t slot;             // partial that the whole job leaves; -1: it writes its result
 };
 static_assert(sizeof(SpaJob) == 48, "three 16-byte loads");
@@ -131,7 +131,7 @@ struct SpaDev {
   int32_t* status;
   float* part_o;            // [slots, 64 groups of 8 columns, 128, 8]: a warp's store of 8 columns is in one piece
   float* part_m;            // [slots, 128] maximum of the scaled scores, log2 units
-  float* part_l;            // [slots, 128] sum relative to it; 0: the row takes no part
+  float* part_l;            // [slots, 128] sum relative to it; 0: the row sees nothing here
   // outputs
   void* out;
   float* softmax_max;
@@ -870,18 +870,11 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const SpaJob& j = w.j;
       const int32_t first = w.tile(), stop = w.stop();
       const int32_t slot = spa_slot(j, first, stop, cluster);
-      // positions that this thread's row sees
-      int32_t vis = 0;
-      if (trow < j.nrows) {
-        const int32_t tok = (j.head0 + trow) / a.p.n1;       // counted from the tile's first token
-        if (!j.packed) vis = a.p.seq.sparse_mode == 3 ? min(j.vis0 + tok, j.hi) : j.hi;
-        else {
-          const int32_t t = (j.row0 + trow) / a.p.n1;
-          const RowInfo ri = row_info(a.p.seq, t);
-          const SpaSeq s = spa_seq(a.p, ri.b, j.hi);
-          if (s.packed && t - s.start < s.act_q) vis = j.hi;
-        }
-      }
+      // positions that this thread's row sees.  Rows that nobody reads (behind the tile's last one, and in a prefix job those of
+      // sequences that are not packed) count as seeing all: masked, they would cost every tile the masks (a tile of 32
+      // rows 20 % more time, and with it the whole call where its pair was the last).
+      int32_t vis = j.hi;
+      if (!j.packed && trow < j.nrows && a.p.seq.sparse_mode == 3) vis = min(j.vis0 + (j.head0 + trow) / a.p.n1, j.hi);
       float m_ref = -INFINITY, m_true = -INFINITY, l = 0.f;
       bool tainted = false;
       for (int32_t t = first; t < stop && ok; ++t, ++n) {
