@@ -8,7 +8,8 @@
 //   - every other sequence is cut into row tiles of its own, each over all the tile's visible keys.  Its tiles are full (or
 //     nearly), so that packing would save nothing; that the prefix is the same pages for everybody then shows as L2 hits.
 // A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into equal
-// shares, one per CTA pair, in the order of the jobs: every pair works for the same time whatever the lengths are.  A job that
+// shares, one per CTA pair, in a line with what each job costs besides: every pair works for about the same time whatever the
+// lengths are.  A job that
 // lies in one pair's share and has no other part writes its result; the others leave normalised fp32 partials
 // (maximum, sum, O) that spa_join_kernel adds up in a fixed order.  One block of rows has
 //   out = sum_i w_i O_i / sum_i w_i,   w_i = l_i exp(m_i - max m).
@@ -63,7 +64,7 @@ constexpr int kSpaPackKeys = 128;    // prefix that can save a tile
 __host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 40 + rows / 8; }
 constexpr int kSpaPlanThreads = 1024;
 constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
-constexpr int kSpaSnapTiles = 3;     // tiles that a share may be longer by so that it ends with its job
+constexpr int kSpaJobTiles = 4;      // what a job costs its pair besides its tiles (Q, the fill of the pipeline, the epilogue), in tiles
 
 constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
 constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
@@ -93,7 +94,7 @@ struct SpaJob {
   int32_t row0, nrows;      // flat rows
   int32_t table_row;        // whose row of the block table the positions are looked up in
   int32_t key0, lo, hi;
-  int32_t tile0, tiles;     // first tile in the order of all jobs' tiles, and their number
+  int32_t tile0, tiles;     // place of its first tile in the line of all jobs' work, and its tiles
   int32_t vis0;             // positions that the first row's token sees (mode 3: one more per token)
   int32_t head0;            // head of the first row
   int32_t packed;           // 1: rows of packed sequences against the prefix (those of other sequences are not read)
@@ -102,10 +103,10 @@ struct SpaJob {
 static_assert(sizeof(SpaJob) == 48, "three 16-byte loads");
 
 struct SpaPlan {
-  int32_t share;                // tiles per CTA pair
+  int32_t share;                // work per CTA pair, in tiles
   int32_t prefix;               // positions shared
 };
-// A CTA pair's share: tiles at .. end - 1, from job `index` on.
+// A CTA pair's share: the tiles at places at .. end - 1 of the line, from job `index` on.
 struct SpaStart {
   int32_t at, end, index, unused;
   SpaJob j;
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
       const int32_t at = jobs + sum_s[0][warp] + x[0] - v[0];
       p.place[f] = make_int2(v[0] ? at : -1, of_seq);
       if (v[0]) {
-        j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1];
+        j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1] + kSpaJobTiles * (at + 1);
         if (v[2]) j.slot = 2 * p.clusters + packed + sum_s[2][warp] + x[2] - v[2];
         p.job[at] = j;
         mine = at;
@@ -339,13 +340,16 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     jobs += total_s[0]; tiles += total_s[1]; packed += total_s[2];
     __syncthreads();
   }
-  int32_t share = max(1, (tiles + p.clusters - 1) / p.clusters);
-  // Few jobs: shares that end with their jobs save a pair its second job (a load of Q, a partial) for tiles that its neighbours
-  // do not have.  Warp w tries shares longer by w tiles; the first that needs no more than one share per pair is
-  // taken: the places of the jobs' tiles are then rounded up to whole shares.
+  // the line: a job's tiles lie behind kSpaJobTiles places for what it costs besides
+  int32_t line = tiles + kSpaJobTiles * jobs;
+  int32_t share = max(1, (line + p.clusters - 1) / p.clusters);
+  // Few jobs: shares that end with their jobs save a pair its second job for tiles that its neighbours do not have.  Warp w tries
+  // shares of w tiles more than the least; the first that needs no more than one share per pair, and is no longer than the
+  // others would be, is taken: the places of the jobs' tiles are then rounded up to whole shares.
   bool single = false;
   if (jobs > 0 && jobs <= kSpaClusters) {
-    const int32_t try_share = share + warp;
+    const int32_t least = max(1, (tiles + p.clusters - 1) / p.clusters);
+    const int32_t try_share = least + warp;
     int32_t parts = 0;
     for (int32_t i = lane; i < jobs; i += 32) parts += (tiles_s[i] + try_share - 1) / try_share;
 #pragma unroll
@@ -353,10 +357,10 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     if (lane == 0) sum_s[0][warp] = parts;
     __syncthreads();
     int32_t extra = 0;
-    while (extra <= kSpaSnapTiles && sum_s[0][extra] > p.clusters) ++extra;
-    if (extra <= kSpaSnapTiles) {
+    while (least + extra <= share && extra < warps && sum_s[0][extra] > p.clusters) ++extra;
+    if (least + extra <= share && extra < warps) {
       single = true;
-      share += extra;
+      share = least + extra;
       if (warp == 0) {
         int32_t before = 0;
         for (int32_t i0 = 0; i0 < jobs; i0 += 32) {
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
         if (lane == 0) total_s[1] = before * share;
       }
       __syncthreads();
-      tiles = total_s[1];
+      line = total_s[1];
     }
   }
   if (tid == 0) {
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     p.plan->prefix = prefix;
   }
   for (int32_t c = tid; c < p.clusters; c += nt)
-    if ((int64_t)c * share >= tiles) p.start[c].at = p.start[c].end = 0;
+    if ((int64_t)c * share >= line) p.start[c].at = p.start[c].end = 0;
   auto deal = [&](int32_t i) {               // job i = j: its place, and the pairs that begin in it
     if (single) {
       j.tile0 = place_s[i];
@@ -391,10 +395,10 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     w.j = j;
     w.index = i;
     w.unused = 0;
-    const int32_t t1 = j.tile0 + j.tiles;
-    for (int32_t c = (j.tile0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
-      w.at = c * share;
-      w.end = min(w.at + share, single ? t1 : tiles);
+    const int32_t t0 = single ? j.tile0 : j.tile0 - kSpaJobTiles, t1 = j.tile0 + j.tiles;
+    for (int32_t c = (t0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
+      w.at = max(c * share, j.tile0);
+      w.end = min((c + 1) * share, single ? t1 : line);
       p.start[c] = w;
     }
   };
@@ -439,11 +443,17 @@ struct SpaWalk {
   __device__ __forceinline__ int32_t tile() const { return at - j.tile0; }                       // of the job
   __device__ __forceinline__ int32_t stop() const { return min(j.tiles, end - j.tile0); }        // tile of the job to stop at
   __device__ __forceinline__ void next_tile() {
-    if (++at < end && at >= j.tile0 + j.tiles) j = spa_load_job(jobs + ++index);
+    if (++at < end && at >= j.tile0 + j.tiles) {
+      j = spa_load_job(jobs + ++index);
+      at = j.tile0;                      // (may lie past the end)
+    }
   }
   __device__ __forceinline__ void next_job() {
     at = j.tile0 + stop();
-    if (at < end) j = spa_load_job(jobs + ++index);
+    if (at < end) {
+      j = spa_load_job(jobs + ++index);
+      at = j.tile0;
+    }
   }
 };
 
@@ -1197,7 +1207,7 @@ inline bool spa_sm100_eligible(const DsaSpaParams* p, int64_t rows) {
   if (p->key_rows >= 0x7FFFFFFF - 256 || rows < 1) return false;
   const SpaWs w = spa_ws_layout(p, rows);
   // tiles of all jobs are counted in 32 bits
-  const int64_t key_tiles = ((int64_t)p->max_blocks * p->block_size + kSpaKeys - 1) / kSpaKeys + 1;
+  const int64_t key_tiles = ((int64_t)p->max_blocks * p->block_size + kSpaKeys - 1) / kSpaKeys + 1 + kSpaJobTiles;
   return (w.prefix_tiles + w.own_tiles) * key_tiles < (1ll << 30);
 }
 
