@@ -57,11 +57,11 @@ constexpr int kSpaThreads = 512;
 constexpr int kSpaQkWarp0 = 3, kSpaSoftWarp0 = 4, kSpaPvWarp = 12, kSpaQkWarp1 = 13, kSpaKWarp1 = 14, kSpaVWarp1 = 15;
 constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
 constexpr int kSpaPackKeys = 128;    // prefix that can save a tile
-// Packing pays when the key tiles that it saves outweigh the partials that it makes, 40 tiles and one per 8 rows.  us a call
-// packed / not: 64 x 64 heads behind 512 keys 46.5 / 39 (saves 128 tiles), 8192 115 / 140 (2048); 32 x 64 heads behind 4096
-// 49 / 55 (512); 64 x 16 heads behind 256 28.5 / 27 (112), 512 28.5 / 31.5 (224), 1024 31.5 / 39.6 (448); 64 x 32 heads
-// behind 4096 53 / 87; 8 x 16 heads behind 512 19.6 / 18.5 (28).
-__host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 40 + rows / 8; }
+// Packing pays when the key tiles that it saves outweigh the partials and jobs that it makes.  us a call packed / not, with the
+// tiles saved: 16 x 8 heads behind 512 keys 24.4 / 22.4 (60), 2048 25.5 / 26.3 (240); 64 x 8 behind 256 33.4 / 30.1 (120),
+// 512 33.0 / 33.2 (240), 2048 34.6 / 50.8 (960); 64 x 16 behind 512 35.1 / 33.3 (224), 1024 34.6 / 39.2 (448); 64 x 32 behind 512
+// 35.5 / 33.4 (192), 1024 36.5 / 39.4 (384); 64 x 64 behind 1024 42.4 / 40.4 (256), 2048 48.0 / 53.1 (512).
+__host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 200 + rows / 32; }
 constexpr int kSpaPlanThreads = 1024;
 constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
 constexpr int kSpaJobTiles = 4;      // what a job costs its pair besides its tiles (Q, the fill of the pipeline, the epilogue), in tiles
