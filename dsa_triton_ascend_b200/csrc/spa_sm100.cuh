@@ -4,41 +4,47 @@
 // Rows.  A row is a (token, head) pair; rows are flat in memory (token * n1 + head), so that 128 consecutive ones are one
 // M = 128 tile whatever the number of heads.  A job is a row tile against a range of key positions:
 //   - where it pays, a sequence of few rows (up to 64) that sees the whole prefix is PACKED: its rows meet the prefix together
-//     with those of its neighbours, in tiles cut from the flat rows of the whole batch (prefix jobs), and its own keys in a job of its own;
+//     with those of its neighbours, in tiles cut from the flat rows of the whole batch (prefix jobs), and its own keys in a
+//     job of its own;
 //   - every other sequence is cut into row tiles of its own, each over all the tile's visible keys.  Its tiles are full (or
 //     nearly), so that packing would save nothing; that the prefix is the same pages for everybody then shows as L2 hits.
-// A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into equal
-// shares, one per CTA pair, in a line with what each job costs besides: every pair works for about the same time whatever the
-// lengths are.  A job that
-// lies in one pair's share and has no other part writes its result; the others leave normalised fp32 partials
-// (maximum, sum, O) that spa_join_kernel adds up in a fixed order.  One block of rows has
+// A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into shares, one per CTA
+// pair, along a line on which every job also takes what it costs besides its tiles: all pairs work for about the same time
+// whatever the lengths are.  A job that lies in one pair's share and has no other part writes its result; the others leave
+// normalised fp32 partials (maximum, sum, O), which spa_join_kernel adds up in a fixed order:
 //   out = sum_i w_i O_i / sum_i w_i,   w_i = l_i exp(m_i - max m).
 //
-// Products.  A CTA pair works on a tile with tcgen05.mma.cta_group::2, M = 128 = 2 x 64 rows: S = Q K^T (N = 128 keys, B
-// split along the keys: CTA c loads keys 64 c .. 64 c + 63 with all 576 features) and O += P V (two N = 256 products per 16
-// keys, B split along the value columns: CTA c loads all 128 keys x columns {c 128 .., 256 + c 128 ..}).  Such a product
-// with A (64 rows a CTA) in shared memory takes 16 + N / 4 cycles per 16 of K: 36 x 48 + 16 x 80 = 3008 cycles for a tile
-// of 128 keys, against 2176 at the full rate and 3584 as two tiles of 64.
-// Tensor memory: lanes 0..63 hold a CTA's rows with the first half of N, lanes 64..127 the same rows with the second:
-// O 256 columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off, so that a score is too small by
-// 5e-7 of itself after 36 steps, and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
+// Products.  A CTA pair works on a tile with tcgen05.mma.cta_group::2, M = 128 = 2 x 64 rows: S = Q K^T (N = 128 keys, B split
+// along the keys: CTA c loads keys 64 c .. 64 c + 63 with all 576 features) and O += P V (two N = 256 products per 16 keys, B
+// split along the value columns: CTA c loads all 128 keys x columns {c 128 .., 256 + c 128 ..}).  Q (72 KB a CTA), a tile of K
+// and three quarters of one of V fill the shared memory; M = 256 would need 144 KB of Q, and O of 128 rows all of tensor memory.
+// Tensor memory: lanes 0..63 hold a CTA's rows with the first half of N, lanes 64..127 the same rows with the second: O 256
+// columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off, so that a score is too small by 5e-7
+// of itself after 36 steps and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
 //
 // Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, as many per box (64, 32, 16, 8) as divide the
 // page size, else with gather4, four rows each.  Absent pages are read at a row past the tensor, which gives zeros without
-// touching memory, and so are the values behind a sequence's end (gathered where they share a group of 8 with
-// others): 0 x NaN would be NaN.  Keys behind the end only make scores that are masked.  Bytes are counted on the even CTA's barriers, where
-// the products are issued.  Rings: K five units of 64 keys x 128 features (the fifth, the rope, 64), one tile,
-// V three units of 32 keys x 256 columns, refilled unit by unit; P has two buffers.
+// touching memory, and so are the values behind a sequence's end (gathered where they share a group of 8 with others):
+// 0 x NaN would be NaN.  Keys behind the end only make scores that are masked.  Bytes are counted on the even CTA's barriers,
+// where the products are issued.  Rings: K five units of 64 keys x 128 features (the fifth, the rope, 64), one tile, V three units
+// of 32 keys x 256 columns, refilled unit by unit; P has two buffers.
 //
-// Softmax.  Eight warps take every tile together: the four threads of a row (two halves of N x two groups of 32 keys)
-// exchange their maxima through shared memory.  P is relative to a running reference that follows the maximum only when it is
-// exceeded by more than 2^8: then O is rescaled in tensor memory (P <= 2^8 fits both types, the sums are fp32).
-// Rows of one tile may see different numbers of keys (causal tokens of one sequence).  A hidden key has P = 0, and
-// 0 x infinity would be NaN: a hidden key whose score is not finite (every non-finite latent makes it so, for every row)
-// marks the token, and sfa_redo_kernel computes it again from its visible keys alone.  Normally no token.
+// Softmax.  Eight warps take every tile together: the four threads of a row (two halves of N x two groups of 32 keys) exchange
+// their maxima through shared memory.  P is relative to a running reference that follows the maximum only when it is
+// exceeded by more than 2^8: then O is rescaled in tensor memory (P <= 2^8 fits both types, the sums are fp32).  P is rounded to
+// the io dtype, the operand type of the second product; its sum is that of the unrounded values.
+// Rows of one tile may see different numbers of keys (causal tokens of one sequence).  A hidden key has P = 0, and 0 x infinity
+// would be NaN: a hidden key whose score is not finite (every non-finite latent makes it so, for every row) marks the
+// token, and sfa_redo_kernel computes it again from its visible keys alone.  Normally no token.
 //
-// Warps (448 threads): 0 K loads, 1 V loads, 2 Q loads and tensor memory, 3 and 13 QK issuers, 4..11 softmax, 12 PV issuer.
-// All waits are bounded; one that gives up sets the status word.
+// What bounds it: 2710 - 2780 cycles per tile of 128 keys, where the products at their full rate take 2176 (tensor pipe 83 %
+// active, issue slots 44 %): 64 x 128 heads behind 16384 + 64 .. 2048 keys 229 us a call in short runs (1360 TFLOP/s, 0.80 of the
+// measured burst rate), 271 under the power cap.  What brought it there, us for that call: one issuer and four loads per block
+// 551; two issuers, wide loads, look-ups a tile ahead 274; two P buffers 246; one thread per loader 238; elected
+// threads (elect.sync; a thread chosen by its number takes twice as long per product) 229.
+//
+// Warps (512 threads): 0 and 14 K loads, 1 and 15 V loads, 2 Q loads and tensor memory, 3 and 13 QK issuers, 4..11 softmax,
+// 12 PV issuer.  All waits are bounded; one that gives up sets the status word.
 #pragma once
 
 #include <algorithm>
@@ -55,16 +61,18 @@ constexpr int kSpaRows = 128;        // rows per tile (64 per CTA)
 constexpr int kSpaKeys = 128;        // keys per tile
 constexpr int kSpaThreads = 512;
 constexpr int kSpaQkWarp0 = 3, kSpaSoftWarp0 = 4, kSpaPvWarp = 12, kSpaQkWarp1 = 13, kSpaKWarp1 = 14, kSpaVWarp1 = 15;
-constexpr int kSpaPackRows = 64;     // a sequence with more rows than this has row tiles of its own
+constexpr int kSpaPackRows = 64;     // a sequence with more rows has row tiles of its own (32 x 96 behind 8192 keys: 92 us packed, 83 not)
 constexpr int kSpaPackKeys = 128;    // prefix that can save a tile
 // Packing pays when the key tiles that it saves outweigh the partials and jobs that it makes.  us a call packed / not, with the
 // tiles saved: 16 x 8 heads behind 512 keys 24.4 / 22.4 (60), 2048 25.5 / 26.3 (240); 64 x 8 behind 256 33.4 / 30.1 (120),
 // 512 33.0 / 33.2 (240), 2048 34.6 / 50.8 (960); 64 x 16 behind 512 35.1 / 33.3 (224), 1024 34.6 / 39.2 (448); 64 x 32 behind 512
 // 35.5 / 33.4 (192), 1024 36.5 / 39.4 (384); 64 x 64 behind 1024 42.4 / 40.4 (256), 2048 48.0 / 53.1 (512).
 __host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 200 + rows / 32; }
-constexpr int kSpaPlanThreads = 1024;
+constexpr int kSpaPlanThreads = 1024;   // 256 where there are no more places: its barriers are cheaper
 constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
-constexpr int kSpaJobTiles = 4;      // what a job costs its pair besides its tiles (Q, the fill of the pipeline, the epilogue), in tiles
+// What a job costs its pair besides its tiles (Q, the fill of the pipeline, the epilogue), in tiles.  64 x 64 heads behind 8192
+// keys, us with 0 .. 6: 114, 102, 90, 83, 80, 81, 83; calls of one job per pair do not mind.
+constexpr int kSpaJobTiles = 4;
 
 constexpr uint32_t kSpaQBlk = 64 * 128;                     // 64 rows x 64 features
 constexpr uint32_t kSpaQBytes = 9 * kSpaQBlk;
