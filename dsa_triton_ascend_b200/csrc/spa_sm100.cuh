@@ -1068,8 +1068,14 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 // one of two), and a tile that its job has written itself is left at once.  A warp joins 16 columns of 32 rows, a row per
 // lane (8 columns of 32 rows are 1 KB in one piece), with four parts' loads in flight; the warps of a block have the same rows
 // and look the parts' maxima and sums up together, while the first O are on their way.
+// kSplit, for few row tiles (whose rows may have a part from every pair): the eight warps have the same columns too and take
+// every eighth part each; their sums meet in shared memory.  The whole call, in us, without and with it: one sequence of 60000
+// keys 62 and 39 (128 heads: 4 groups of 32 rows); 4 such of 16000 keys 40 and 36 (16 groups); 6 and 8 of them 46 and 46, 51
+// and 54 (24 and 32 groups); 8 heads behind a prefix of 8192 keys, 16 sequences 32 and 29, 20 of them 31 and 33 (20 groups).
 constexpr int kSpaJoinThreads = 256;
-constexpr int kSpaJoinBlocks = (kSpaRows / 32) * (512 / 16) / (kSpaJoinThreads / 32);   // blocks of a row tile, a task per warp
+constexpr int kSpaJoinWarps = kSpaJoinThreads / 32;
+constexpr int kSpaJoinFew = 16;                                 // row groups of 32 up to which parts are split over warps
+constexpr int kSpaJoinTasks = (kSpaRows / 32) * (512 / 16);     // of 32 rows x 16 columns in a row tile
 struct SpaParts { int32_t first, count, uncut; };      // first share, number of shares, partial of a job in one share
 __device__ __forceinline__ SpaParts spa_parts(const SpaDev& p, int32_t job, int32_t share) {
   SpaParts w = {0, 0, -1};
@@ -1081,8 +1087,10 @@ __device__ __forceinline__ SpaParts spa_parts(const SpaDev& p, int32_t job, int3
   }
   return w;
 }
+template <bool kSplit>
 __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaDev p, int32_t is_bf16) {
   __shared__ float2 ml_s[2 * kSpaClusters + 2][32];      // (maximum, sum) of part, row
+  static_assert(sizeof(ml_s) >= kSpaJoinWarps * 17 * 32 * 4, "the warps' sums");
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31;
@@ -1104,9 +1112,12 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
     if ((row0 + total - 1) / kSpaRows > pre0) pre[1] = spa_parts(p, p.place[pre0 + 1].x, share);
   }
   const int warp = threadIdx.x >> 5;
-  for (int32_t y = blockIdx.y; y < kSpaJoinBlocks; y += gridDim.y) {
-    const int32_t r = (y >> 2) * 32 + lane, cols = ((y & 3) * 8 + warp) * 16;
-    if ((y >> 2) * 32 >= total) break;
+  for (int32_t y = blockIdx.y; y < kSpaJoinTasks / (kSplit ? 1 : kSpaJoinWarps); y += gridDim.y) {
+    const int32_t task = kSplit ? y : y * kSpaJoinWarps + warp;
+    const int32_t r = (task >> 5) * 32 + lane, cols = (task & 31) * 16;
+    if ((task >> 5) * 32 >= total) break;
+    constexpr int kStep = kSplit ? kSpaJoinWarps : 1;     // from a part of this warp to its next
+    const int32_t part0 = kSplit ? warp : 0;
     const bool todo = r < total && !(written && r < active);
     const int32_t row = row0 + min(r, total - 1), prow = row % kSpaRows;
     const bool second = row / kSpaRows > pre0;
@@ -1125,17 +1136,18 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
     auto load = [&](int32_t k0) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (k0 + e >= parts) continue;
+        const int32_t k = k0 + e * kStep;
+        if (k >= parts) continue;
         int32_t tr;
-        const int64_t slot = at(k0 + e, tr);
+        const int64_t slot = at(k, tr);
         const float* o = p.part_o + ((slot * 64 + cols / 8) * kSpaRows + tr) * 8;
         ptx::ld_global_v8(o, v[e]);
         ptx::ld_global_v8(o + kSpaRows * 8, v[e] + 8);
       }
     };
-    load(0);
+    load(part0);
     __syncthreads();               // (the turn before has read ml_s)
-    for (int32_t k = warp; k < parts; k += kSpaJoinThreads / 32) {
+    for (int32_t k = warp; k < parts; k += kSpaJoinWarps) {
       int32_t tr;
       const int64_t i = at(k, tr) * kSpaRows + tr;
       ml_s[k][lane] = make_float2(p.part_m[i], p.part_l[i]);
@@ -1147,17 +1159,32 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
       if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
     }
     float acc[16] = {}, den = 0.f;
-    for (int32_t k0 = 0; k0 < parts; k0 += 4) {
-      if (k0 > 0) load(k0);
+    for (int32_t k0 = part0; k0 < parts; k0 += 4 * kStep) {
+      if (k0 > part0) load(k0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (k0 + e >= parts) continue;
-        const float2 ml = ml_s[k0 + e][lane];
+        if (k0 + e * kStep >= parts) continue;
+        const float2 ml = ml_s[k0 + e * kStep][lane];
         if (ml.y == 0.f) continue;           // (its O may never have been written)
         const float f = ml.y * ex2(ml.x - mx);
         den += f;
 #pragma unroll
         for (int c = 0; c < 16; ++c) acc[c] += f * v[e][c];
+      }
+    }
+    if (kSplit) {
+      float* sum = reinterpret_cast<float*>(ml_s);        // [8 warps][17][32]
+      __syncthreads();                                    // (everybody has read the weights)
+#pragma unroll
+      for (int c = 0; c < 16; ++c) sum[(warp * 17 + c) * 32 + lane] = acc[c];
+      sum[(warp * 17 + 16) * 32 + lane] = den;
+      __syncthreads();
+      if (warp != 0) continue;
+#pragma unroll 1
+      for (int w = 1; w < kSpaJoinWarps; ++w) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) acc[c] += sum[(w * 17 + c) * 32 + lane];
+        den += sum[(w * 17 + 16) * 32 + lane];
       }
     }
     if (!todo) continue;
@@ -1306,8 +1333,14 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
       cudaSuccess)
     return DSA_ERR_CUDA;
   // a task per warp, more where there are so many tiles that most are written by their jobs
-  const dim3 join_grid((unsigned)w.own_tiles, w.own_tiles <= 512 ? kSpaJoinBlocks : 1);
-  if (launch_after(spa_join_kernel, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16) != cudaSuccess)
+  const int64_t seq_rows = w.own_tiles_per_seq > 0 ? (int64_t)p->s1 * p->n1 : (int64_t)rows;
+  const int64_t tile_rows = std::min<int64_t>(kSpaRows, seq_rows);
+  const int64_t groups = (tile_rows + 31) / 32;              // of 32 rows in a tile, at most
+  const bool few = w.own_tiles * groups <= kSpaJoinFew;
+  const dim3 join_grid((unsigned)w.own_tiles,
+                       few ? (unsigned)groups * (512 / 16) : w.own_tiles <= 512 ? kSpaJoinTasks / kSpaJoinWarps : 1);
+  if ((few ? launch_after(spa_join_kernel<true>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16)
+           : launch_after(spa_join_kernel<false>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16)) != cudaSuccess)
     return DSA_ERR_CUDA;
   count_launch(3);
   if (w.redo_used) {

@@ -429,6 +429,21 @@ def test_lengths_past_the_table(kind):
     assert torch.isnan(got[0][0]).all() and torch.isfinite(got[0][1:]).all()
 
 
+@pytest.mark.parametrize("heads", [3, 33, 70, 128])
+@pytest.mark.parametrize("batch,length", [(1, 20000), (1, 9473), (2, 12000), (3, 7001), (4, 6100), (5, 5200), (9, 3500)])
+def test_few_rows_in_many_parts(heads, batch, length):
+    """Rows with parts from one share, from every share, and from a few, with the parts joined by one warp and by eight."""
+    verify(make(heads + batch, "BSND", [1] * batch, [length - 131 * i for i in range(batch)], heads, 64, 0), "tensor")
+
+
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
+@pytest.mark.parametrize("batch", [1, 2, 8, 16, 17])
+def test_few_packed_rows_in_many_parts(layout, batch):
+    s = make(batch, layout, [1 + b % 2 for b in range(batch)], [9000 + 37 * b for b in range(batch)], 8, 64, 8192)
+    a, b = verify(s, "tensor"), verify(s, "tensor")
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 @pytest.mark.parametrize("kind", KERNELS)
 @pytest.mark.parametrize("heads", [16, 128])
 def test_a_query_that_is_not_a_number_spoils_its_own_row_only(kind, heads):
