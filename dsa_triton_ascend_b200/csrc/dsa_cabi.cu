@@ -1037,7 +1037,7 @@ int dsa_spa_forward(const DsaSpaParams* p, void* workspace, size_t workspace_byt
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u) != 0) return DSA_ERR_WORKSPACE;
   if (p->kernel == DSA_KERNEL_TENSOR && !dsa_spa_uses_tensor_path(p)) return DSA_ERR_UNSUPPORTED;
   cudaStream_t cs = (cudaStream_t)stream;
-  if (dsa_spa_uses_tensor_path(p))   // (the plan kernel clears the header)
+  if (dsa_spa_uses_tensor_path(p))   // (its kernels write the header)
     return spa_sm100_launch(p, spa_dense_dev(p), (int32_t*)workspace, (char*)workspace + kWorkspaceHeader, cs);
   if (cudaMemsetAsync(workspace, 0, kWorkspaceHeader, cs) != cudaSuccess) return DSA_ERR_CUDA;
   if (spa_rows(p) == 0) return DSA_OK;

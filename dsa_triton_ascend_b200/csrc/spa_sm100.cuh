@@ -8,9 +8,9 @@
 //     job of its own;
 //   - every other sequence is cut into row tiles of its own, each over all the tile's visible keys.  Its tiles are full (or
 //     nearly), so that packing would save nothing; that the prefix is the same pages for everybody then shows as L2 hits.
-// A plan kernel lists the jobs (the lengths live on the device) and cuts their key tiles, 128 keys each, into shares, one per CTA
-// pair, along a line on which every job also takes what it costs besides its tiles: all pairs work for about the same time
-// whatever the lengths are.  A job that lies in one pair's share and has no other part writes its result; the others leave
+// A plan (a kernel, or with few jobs every CTA for itself) lists the jobs (the lengths live on the device) and cuts their key
+// tiles, 128 keys each, into shares, one per CTA pair, along a line on which every job also takes what it costs besides its
+// tiles: all pairs work for about the same time whatever the lengths are.  A job that lies in one pair's share and has no other part writes its result; the others leave
 // normalised fp32 partials (maximum, sum, O), which spa_join_kernel adds up in a fixed order:
 //   out = sum_i w_i O_i / sum_i w_i,   w_i = l_i exp(m_i - max m).
 //
@@ -69,6 +69,10 @@ constexpr int kSpaPackKeys = 128;    // prefix that can save a tile
 // 35.5 / 33.4 (192), 1024 36.5 / 39.4 (384); 64 x 64 behind 1024 42.4 / 40.4 (256), 2048 48.0 / 53.1 (512).
 __host__ __device__ constexpr int64_t spa_pack_least(int64_t rows) { return 200 + rows / 32; }
 constexpr int kSpaPlanThreads = 1024;   // 256 where there are no more places: its barriers are cheaper
+// Places up to which every CTA of the main kernel plans for itself, which saves a launch: 8 x 8 heads 28.1 us of the host against 25.6,
+// the GPU's side 20.4 / 20.7; one sequence of 60000 keys 39 / 36 on the GPU, 16 x 16 heads over 16000 keys 74.4 / 75.8, 64 x 16
+// heads behind 16384 (72 places) 63.6 / 65.6.
+constexpr int kSpaPlanEach = 64;
 constexpr int kSpaClusters = 74;     // shares of the work (the workspace size must not depend on the device)
 // What a job costs its pair besides its tiles (Q, the fill of the pipeline, the epilogue), in tiles.  64 x 64 heads behind 8192
 // keys, us with 0 .. 6: 114, 102, 90, 83, 80, 81, 83; calls of one job per pair do not mind.
@@ -133,6 +137,7 @@ struct SpaDev {
   int32_t prefix_tiles, own_tiles, own_tiles_per_seq;   // places in the list of row tiles (own_tiles_per_seq: BSND)
   int32_t pack_rows;        // kSpaPackRows, or 0 when nothing may be packed
   int32_t clusters;
+  int32_t places_each;      // > 0: every CTA of the main kernel plans for itself, with room for so many jobs; 0: a plan kernel
   // workspace
   SpaPlan* plan;
   SpaJob* job;              // [prefix_tiles + own_tiles]
@@ -142,6 +147,7 @@ struct SpaDev {
   int32_t* redo_list;       // [rows]
   int32_t* redo_count;
   int32_t* status;
+  int32_t* fail;            // [2 clusters] CTAs that plan for themselves: what they have to say in place of the status
   float* part_o;            // [slots, 64 groups of 8 columns, 128, 8]: a warp's store of 8 columns is in one piece
   float* part_m;            // [slots, 128] maximum of the scaled scores, log2 units
   float* part_l;            // [slots, 128] sum relative to it; 0: the row sees nothing here
@@ -191,21 +197,24 @@ __device__ __forceinline__ int32_t spa_own_place(const SpaDev& p, int32_t b, int
   return (int32_t)((int64_t)start * p.n1 / kSpaRows) + b;
 }
 
-// ---- plan: one block ------------------------------------------------------------------------------
-__global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev p) {
-  __shared__ unsigned long long best_s[32];
-  __shared__ int32_t sum_s[3][33];
-  __shared__ int32_t total_s[3];
-  __shared__ int32_t tiles_s[kSpaClusters], place_s[kSpaClusters];   // of the first jobs: tiles, and their place
+// ---- plan: one block -----------------------------------------------------------------------------------
+struct SpaPlanSmem {
+  unsigned long long best_s[32];
+  int32_t sum_s[3][33];
+  int32_t total_s[3];
+  int32_t tiles_s[kSpaClusters], place_s[kSpaClusters];   // of the first jobs: tiles, and their place
+};
+// cluster < 0: a kernel of its own, which leaves every pair's start.  Otherwise for the pair `cluster` by each of its CTAs: its start
+// in `start`, the jobs of its share in `own_jobs`; `publish`: one CTA leaves what the join reads.
+__device__ __noinline__ void spa_plan(const SpaDev& p, SpaPlanSmem& sm, int32_t cluster, SpaStart* start, SpaJob* own_jobs,
+                                      bool publish) {
+  auto& best_s = sm.best_s;
+  auto& sum_s = sm.sum_s;
+  auto& total_s = sm.total_s;
+  auto& tiles_s = sm.tiles_s;
+  auto& place_s = sm.place_s;
   const int nt = blockDim.x, warps = nt >> 5;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  grid_dep_launch();
-  grid_dep_wait();
-  if (tid < 64) p.status[tid] = 0;
-  if (p.redo != nullptr) {
-    if (tid == 0) *p.redo_count = 0;
-    for (int32_t i = tid; i < p.rows; i += nt) p.redo[i] = 0;
-  }
   // the longest sequence (the first of them) lends its pages for the prefix
   int32_t prefix = 0, ref = 0;
   if (p.pack_rows > 0) {
@@ -340,11 +349,11 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
     __syncthreads();
     if (f < places) {
       const int32_t at = jobs + sum_s[0][warp] + x[0] - v[0];
-      p.place[f] = make_int2(v[0] ? at : -1, of_seq);
+      if (publish) p.place[f] = make_int2(v[0] ? at : -1, of_seq);
       if (v[0]) {
         j.tile0 = tiles + sum_s[1][warp] + x[1] - v[1] + kSpaJobTiles * (at + 1);
         if (v[2]) j.slot = 2 * p.clusters + packed + sum_s[2][warp] + x[2] - v[2];
-        p.job[at] = j;
+        if (publish) p.job[at] = j;
         mine = at;
         if (at < kSpaClusters) tiles_s[at] = j.tiles;
       }
@@ -392,36 +401,59 @@ __global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const SpaDev 
       line = total_s[1];
     }
   }
-  if (tid == 0) {
+  if (tid == 0 && publish) {
     p.plan->share = share;
     p.plan->prefix = prefix;
   }
-  for (int32_t c = tid; c < p.clusters; c += nt)
-    if ((int64_t)c * share >= line) p.start[c].at = p.start[c].end = 0;
+  if (cluster < 0) {
+    for (int32_t c = tid; c < p.clusters; c += nt)
+      if ((int64_t)c * share >= line) p.start[c].at = p.start[c].end = 0;
+  } else if (tid == 0 && (int64_t)cluster * share >= line) {
+    start->at = start->end = 0;
+  }
   auto deal = [&](int32_t i) {               // job i = j: its place, and the pairs that begin in it
     if (single) {
       j.tile0 = place_s[i];
-      p.job[i].tile0 = j.tile0;
+      if (publish) p.job[i].tile0 = j.tile0;
     }
     SpaStart w;
     w.j = j;
     w.index = i;
     w.unused = 0;
     const int32_t t0 = single ? j.tile0 : j.tile0 - kSpaJobTiles, t1 = j.tile0 + j.tiles;
-    for (int32_t c = (t0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) {
+    auto begin = [&](int32_t c, SpaStart& to) {
       w.at = max(c * share, j.tile0);
       w.end = min((c + 1) * share, single ? t1 : line);
-      p.start[c] = w;
+      to = w;
+    };
+    if (cluster < 0) {
+      for (int32_t c = (t0 + share - 1) / share; c < p.clusters && c * share < t1; ++c) begin(c, p.start[c]);
+    } else {
+      const int32_t at = cluster * share;
+      if (at >= t0 && at < t1) begin(cluster, *start);
+      if (t0 < at + share && t1 > at) own_jobs[i] = j;
     }
   };
   if (places <= nt) {                        // (the jobs are still at hand)
     if (mine >= 0) deal(mine);
   } else {
-    for (int32_t i = tid; i < jobs; i += nt) {
+    for (int32_t i = tid; i < jobs; i += nt) {   // (a kernel of its own)
       j = p.job[i];
       deal(i);
     }
   }
+}
+__global__ void __launch_bounds__(kSpaPlanThreads) spa_plan_kernel(const __grid_constant__ SpaDev p) {
+  __shared__ SpaPlanSmem sm;
+  const int tid = threadIdx.x;
+  grid_dep_launch();
+  grid_dep_wait();
+  if (tid < 64) p.status[tid] = 0;
+  if (p.redo != nullptr) {
+    if (tid == 0) *p.redo_count = 0;
+    for (int32_t i = tid; i < p.rows; i += blockDim.x) p.redo[i] = 0;
+  }
+  spa_plan(p, sm, -1, nullptr, nullptr, true);
 }
 
 // Where the tiles a .. b - 1 of a job leave their result: -1 in the output, else a partial.  A pair's share has at most one
@@ -443,11 +475,11 @@ struct SpaWalk {
   const SpaJob* jobs;
   int32_t at, end, index;
   SpaJob j;
-  __device__ __forceinline__ void start(const SpaDev& p, int32_t cluster) {
-    jobs = p.job;
+  __device__ __forceinline__ void start(const SpaJob* list, const SpaStart* from) {
+    jobs = list;
     SpaStart w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&w)[i] = reinterpret_cast<const int4*>(p.start + cluster)[i];
+    for (int i = 0; i < 4; ++i) reinterpret_cast<int4*>(&w)[i] = reinterpret_cast<const int4*>(from)[i];
     at = w.at; end = w.end; index = w.index;
     j = w.j;
   }
@@ -498,7 +530,9 @@ struct SpaLoads {
   uint64_t *full, *empty;
   uint32_t full_lead;          // full[0] of the even CTA
   uint32_t dst;
-  int32_t rank, cluster;
+  const SpaJob* jobs;
+  const SpaStart* start;
+  int32_t rank;
   int32_t u0;                  // first unit
   volatile int* abort_flag;
 };
@@ -509,7 +543,7 @@ template <int kBoxes>
 __device__ __forceinline__ void spa_k_boxes(const SpaArgs& a, const SpaLoads& o) {
   constexpr int kKeys = 64 / kBoxes;
   SpaWalk w;
-  w.start(a.p, o.cluster);
+  w.start(o.jobs, o.start);
   SpaSpot spot[kBoxes];
   auto look_up = [&]() {
     if (!w.more()) return;
@@ -551,7 +585,7 @@ template <int kBoxes>
 __device__ __forceinline__ void spa_v_boxes(const SpaArgs& a, const SpaLoads& o) {
   constexpr int kKeys = 32 / kBoxes;
   SpaWalk w;
-  w.start(a.p, o.cluster);
+  w.start(o.jobs, o.start);
   SpaSpot spot[2][kBoxes];
   int32_t first = 0, lo = 0, hi = 0;          // position of the tile, and what is wanted
   auto look_up = [&]() {
@@ -620,7 +654,7 @@ template <bool kV>
 __device__ __forceinline__ void spa_gather(const SpaArgs& a, const SpaLoads& o) {
   const int lane = threadIdx.x & 31;
   SpaWalk w;
-  w.start(a.p, o.cluster);
+  w.start(o.jobs, o.start);
   SpaSpot spot[4];
   auto look_up = [&]() {
     if (!w.more()) return;
@@ -675,7 +709,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                      const __grid_constant__ CUtensorMap tmap_kh, const __grid_constant__ CUtensorMap tmap_rh,
                      const __grid_constant__ CUtensorMap tmap_k1, const __grid_constant__ CUtensorMap tmap_r1,
                      const __grid_constant__ CUtensorMap tmap_vh, const __grid_constant__ CUtensorMap tmap_v8,
-                     const SpaArgs a) {
+                     const __grid_constant__ SpaArgs a) {
   extern __shared__ __align__(1024) unsigned char spa_sm[];
   unsigned char* q_s = spa_sm + kSpaOffQ;
   unsigned char* k_s = spa_sm + kSpaOffK;
@@ -729,6 +763,17 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   grid_dep_launch();
   grid_dep_wait();           // (nothing before this touches global memory)
   const uint32_t tmem = *tmem_slot;
+  const SpaJob* jobs = a.p.job;
+  const SpaStart* start = a.p.start + cluster;
+  if (a.p.places_each > 0) {
+    SpaStart* own_start = reinterpret_cast<SpaStart*>(spa_sm + kSpaOffBar + 256);
+    SpaJob* own_jobs = a.p.job + (int64_t)a.p.places_each * (1 + blockIdx.x);
+    static_assert(sizeof(SpaPlanSmem) <= 2048 && sizeof(SpaStart) <= 256, "in place of the maxima, and behind the barriers");
+    spa_plan(a.p, *reinterpret_cast<SpaPlanSmem*>(spa_sm + kSpaOffX), cluster, own_start, own_jobs, blockIdx.x == 0);
+    __syncthreads();
+    jobs = own_jobs;
+    start = own_start;
+  }
 
   if (*abort_flag) {
     // nothing started
@@ -738,7 +783,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     SpaLoads o;
     o.box = &tmap_kh; o.box8 = nullptr; o.rope = &tmap_rh; o.gather = &tmap_k1; o.rope_gather = &tmap_r1;
     o.full = k_full; o.empty = k_empty; o.full_lead = ptx::map_to_rank(&k_full[0], 0);
-    o.dst = ptx::smem_u32(k_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 0 ? 0 : 2; o.abort_flag = abort_flag;
+    o.dst = ptx::smem_u32(k_s); o.rank = (int32_t)rank; o.jobs = jobs; o.start = start; o.u0 = warp == 0 ? 0 : 2; o.abort_flag = abort_flag;
     if (a.box_keys == 0) spa_gather<false>(a, o);
     else if (ptx::elect_one()) {
       if (a.box_keys == 64) spa_k_boxes<1>(a, o);
@@ -752,7 +797,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     SpaLoads o;
     o.box = &tmap_vh; o.box8 = &tmap_v8; o.rope = nullptr; o.gather = &tmap_k1; o.rope_gather = nullptr;
     o.full = v_full; o.empty = v_empty; o.full_lead = ptx::map_to_rank(&v_full[0], 0);
-    o.dst = ptx::smem_u32(v_s); o.rank = (int32_t)rank; o.cluster = cluster; o.u0 = warp == 1 ? 0 : 1; o.abort_flag = abort_flag;
+    o.dst = ptx::smem_u32(v_s); o.rank = (int32_t)rank; o.jobs = jobs; o.start = start; o.u0 = warp == 1 ? 0 : 1; o.abort_flag = abort_flag;
     if (a.box_keys == 0) spa_gather<true>(a, o);
     else if (ptx::elect_one()) {
       if (a.box_keys >= 32) spa_v_boxes<1>(a, o);
@@ -763,7 +808,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     // ------------------------------------------------------------------ Q loads
     if (lane == 0) {
       SpaWalk w;
-      w.start(a.p, cluster);
+      w.start(jobs, start);
       bool ok = true;
       const uint32_t bar = ptx::map_to_rank(q_full, 0);
       for (uint32_t n = 0; w.more() && ok; ++n, w.next_job()) {
@@ -784,7 +829,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       const bool second = warp == kSpaQkWarp1;      // units 2 and 3; the first: 0, 1 and the rope
       const int units = second ? 2 : 3;
       SpaWalk w;
-      w.start(a.p, cluster);
+      w.start(jobs, start);
       bool ok = true;
       const uint64_t qd = ptx::desc_kmajor_sw128(ptx::smem_u32(q_s)), kd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s), 2048);
       const uint64_t rd = ptx::desc_kmajor_sw128(ptx::smem_u32(k_s));
@@ -822,7 +867,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     // ------------------------------------------------------------------ PV issuer
     if (rank == 0 && ptx::elect_one()) {
       SpaWalk w;
-      w.start(a.p, cluster);
+      w.start(jobs, start);
       bool ok = true;
       const uint64_t pd = ptx::desc_kmajor_sw128(ptx::smem_u32(p_s)), vd = ptx::desc_mnmajor_sw128(ptx::smem_u32(v_s), 1024, 4096);
       const uint32_t p_hi = (uint32_t)(pd >> 32), v_hi = (uint32_t)(vd >> 32);
@@ -887,7 +932,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       return got;
     };
     SpaWalk w;
-    w.start(a.p, cluster);
+    w.start(jobs, start);
     for (; w.more() && ok; w.next_job()) {
       const SpaJob& j = w.j;
       const int32_t first = w.tile(), stop = w.stop();
@@ -1064,7 +1109,10 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     ptx::tc_fence_after();
     ptx::tmem_dealloc_pair(tmem, 512);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicExch(a.p.status, misaligned ? 2 : 1);
+  if (threadIdx.x == 0) {
+    if (a.p.places_each > 0) a.p.fail[blockIdx.x] = *abort_flag;
+    else if (*abort_flag) atomicExch(a.p.status, misaligned ? 2 : 1);
+  }
 }
 
 // ---- join: the rows whose result is in parts, or that see nothing ----------------------------------
@@ -1098,6 +1146,10 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
   grid_dep_launch();
   grid_dep_wait();
   const int lane = threadIdx.x & 31;
+  if (p.places_each > 0 && blockIdx.x == 0 && blockIdx.y == 0) {     // (otherwise the plan kernel and the main one have seen to it)
+    const int bad = __syncthreads_or(threadIdx.x < 2 * kSpaClusters && p.fail[threadIdx.x] != 0);
+    if (threadIdx.x < 64) p.status[threadIdx.x] = threadIdx.x == 0 && bad ? 1 : 0;
+  }
   const int32_t share = p.plan->share, prefix = p.plan->prefix;
   const int2 mine = p.place[p.prefix_tiles + blockIdx.x];
   const SpaSeq s = spa_seq(p, mine.y, prefix);
@@ -1208,8 +1260,8 @@ __global__ void __launch_bounds__(kSpaJoinThreads, 2) spa_join_kernel(const SpaD
 
 // ---- host side ---------------------------------------------------------------------------------
 struct SpaWs {
-  size_t plan, job, place, start, redo, redo_list, redo_count, part_m, part_l, part_o, total;
-  int64_t prefix_tiles, own_tiles, own_tiles_per_seq, slots;
+  size_t plan, job, place, start, fail, redo, redo_list, redo_count, part_m, part_l, part_o, total;
+  int64_t prefix_tiles, own_tiles, own_tiles_per_seq, slots, places_each;
   bool pack, redo_used;
 };
 inline SpaWs spa_ws_layout(const DsaSpaParams* p, int64_t rows) {
@@ -1229,9 +1281,11 @@ inline SpaWs spa_ws_layout(const DsaSpaParams* p, int64_t rows) {
   const size_t places = (size_t)(w.prefix_tiles + w.own_tiles);
   w.plan = 0;
   w.job = 256;
-  w.place = w.job + up(places * sizeof(SpaJob));
+  w.places_each = places <= kSpaPlanEach && !w.redo_used ? (int64_t)places : 0;
+  w.place = w.job + up(places * sizeof(SpaJob) * (w.places_each > 0 ? 1 + 2 * kSpaClusters : 1));
   w.start = w.place + up(places * 8);
-  w.redo_count = w.start + up(kSpaClusters * sizeof(SpaStart));
+  w.fail = w.start + up(kSpaClusters * sizeof(SpaStart));
+  w.redo_count = w.fail + up(2 * kSpaClusters * 4);
   w.redo = w.redo_count + 256;
   w.redo_list = w.redo + (w.redo_used ? up((size_t)rows * 4) : 0);
   w.part_m = w.redo_list + (w.redo_used ? up((size_t)rows * 4) : 0);
@@ -1297,8 +1351,9 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   d.prefix_tiles = (int32_t)w.prefix_tiles; d.own_tiles = (int32_t)w.own_tiles; d.own_tiles_per_seq = (int32_t)w.own_tiles_per_seq;
   d.pack_rows = w.pack ? kSpaPackRows : 0;
   d.clusters = kSpaClusters;
+  d.places_each = (int32_t)w.places_each;
   d.plan = (SpaPlan*)(ws + w.plan); d.job = (SpaJob*)(ws + w.job); d.place = (int2*)(ws + w.place);
-  d.start = (SpaStart*)(ws + w.start);
+  d.start = (SpaStart*)(ws + w.start); d.fail = (int32_t*)(ws + w.fail);
   d.redo = w.redo_used ? (int32_t*)(ws + w.redo) : nullptr;
   d.redo_list = (int32_t*)(ws + w.redo_list); d.redo_count = (int32_t*)(ws + w.redo_count);
   d.status = status;
@@ -1331,7 +1386,7 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
     return DSA_ERR_CUDA;
   // (barriers of 8 warps are cheaper than those of 32)
   const int plan_threads = w.prefix_tiles + w.own_tiles <= 256 ? 256 : kSpaPlanThreads;
-  if (launch_after(spa_plan_kernel, dim3(1), dim3(plan_threads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
+  if (w.places_each == 0 && launch_after(spa_plan_kernel, dim3(1), dim3(plan_threads), 0, st, d) != cudaSuccess) return DSA_ERR_CUDA;
   if (launch_after(spa_fwd_sm100_kernel, dim3(2 * kSpaClusters), dim3(kSpaThreads), kSpaSmemBytes, st, q, qr, kh, rh, k1, r1,
                    vh, v8, a) !=
       cudaSuccess)
@@ -1346,7 +1401,7 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   if ((few ? launch_after(spa_join_kernel<true>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16)
            : launch_after(spa_join_kernel<false>, dim3(join_grid), dim3(kSpaJoinThreads), 0, st, d, a.is_bf16)) != cudaSuccess)
     return DSA_ERR_CUDA;
-  count_launch(3);
+  count_launch(w.places_each > 0 ? 2 : 3);
   if (w.redo_used) {
     const size_t smem = (size_t)(kSfaSimtHeads + kSfaSimtKeys) * (p->d + p->d_rope + kSfaSimtPad) * 2;
     const int64_t work = (int64_t)d.rows * ((p->n1 + kSfaSimtHeads - 1) / kSfaSimtHeads);
