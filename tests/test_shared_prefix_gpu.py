@@ -437,6 +437,15 @@ def test_few_rows_in_many_parts(heads, batch, length):
 
 
 @pytest.mark.parametrize("layout", ["BSND", "TND"])
+@pytest.mark.parametrize("prefix", [0, 640])
+@pytest.mark.parametrize("batch", [31, 58, 60, 61, 62, 63, 64, 65, 80])
+def test_around_the_row_tiles_that_are_planned_without_a_kernel(layout, prefix, batch):
+    """One token and eight heads a sequence; some sequences without keys, or with fewer than the prefix."""
+    kv = [prefix + (b * 37) % 290 if b % 7 else b % 3 * 100 for b in range(batch)]
+    verify(make(batch, layout, [1] * batch, kv, 8, 64, prefix), "tensor")
+
+
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
 @pytest.mark.parametrize("batch", [1, 2, 8, 16, 17])
 def test_few_packed_rows_in_many_parts(layout, batch):
     s = make(batch, layout, [1 + b % 2 for b in range(batch)], [9000 + 37 * b for b in range(batch)], 8, 64, 8192)
