@@ -198,7 +198,8 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
         const float m_old = m_s[h];
         if (two_pass && pass == 1) {
           const float l = l_s[h];
-          const float pv = (valid && l > 0.f) ? expf(sv - m_old) / l : 0.f;
+          // (dense: a sum that is not a number makes the whole row none)
+          const float pv = (valid && (kDense ? l != 0.f : l > 0.f)) ? expf(sv - m_old) / l : 0.f;
           pt[h * PK + lane] = from_f32<T>(pv);
           if (lane == 0) alpha_s[h] = 1.f;
           continue;
@@ -252,7 +253,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
       const int h = g + half * 8;
       if (h0 + h >= p.n1) continue;
       const float l = l_s[h];
-      const float inv = two_pass ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+      const float inv = two_pass ? 1.f : ((kDense ? l != 0.f : l > 0.f) ? 1.f / l : 0.f);
       T* o = outp + (int64_t)h * p.d;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
