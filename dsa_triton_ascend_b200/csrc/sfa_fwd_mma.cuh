@@ -71,7 +71,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c4 = lane & 3;
   const RowInfo ri = row_info(p.seq, row);
-  const bool row_active = ri.pos < ri.act_q && ri.threshold > 0 && ri.act_k > 0;
+  const bool row_active = kDense ? ri.visible > 0 : ri.pos < ri.act_q && ri.threshold > 0 && ri.act_k > 0;
 
   // output accumulator: heads g and g + 8, d / 64 column tiles of 8 per warp (warp w: columns
   // (d / 8) w .. (d / 8) (w + 1) - 1), in the mma accumulator layout
@@ -198,8 +198,9 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
         const float m_old = m_s[h];
         if (two_pass && pass == 1) {
           const float l = l_s[h];
-          // (dense: a sum that is not a number makes the whole row none)
-          const float pv = (valid && (kDense ? l != 0.f : l > 0.f)) ? expf(sv - m_old) / l : 0.f;
+          // (dense: every row here sees a key; a sum that is not a number, or that is zero because all scores are minus
+          // infinity, makes the whole row none)
+          const float pv = (valid && (kDense || l > 0.f)) ? expf(sv - m_old) / l : 0.f;
           pt[h * PK + lane] = from_f32<T>(pv);
           if (lane == 0) alpha_s[h] = 1.f;
           continue;
@@ -253,7 +254,8 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
       const int h = g + half * 8;
       if (h0 + h >= p.n1) continue;
       const float l = l_s[h];
-      const float inv = two_pass ? 1.f : ((kDense ? l != 0.f : l > 0.f) ? 1.f / l : 0.f);
+      // (dense, l = 0: the accumulator is zero or NaN, and its product with infinity is NaN)
+      const float inv = two_pass ? 1.f : (kDense || l > 0.f ? 1.f / l : 0.f);
       T* o = outp + (int64_t)h * p.d;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
@@ -266,10 +268,10 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
     }
     if (p.return_lse && tid < kSfaSimtHeads && h0 + tid < p.n1) {
       const float lt = l_s[tid];
-      // (dense: a row whose sum is not a number says so)
-      const bool nan = kDense && lt != lt;
-      p.softmax_max[(int64_t)row * p.n1 + h0 + tid] = nan ? lt : lt > 0.f ? m_s[tid] : 0.f;
-      p.softmax_sum[(int64_t)row * p.n1 + h0 + tid] = nan ? lt : lt > 0.f ? lt : 0.f;
+      // (dense: a row whose sum is not a number, or is none, says so)
+      const float none = kDense ? nanf("") : 0.f;
+      p.softmax_max[(int64_t)row * p.n1 + h0 + tid] = lt > 0.f ? m_s[tid] : none;
+      p.softmax_sum[(int64_t)row * p.n1 + h0 + tid] = lt > 0.f ? lt : none;
     }
   }
 }

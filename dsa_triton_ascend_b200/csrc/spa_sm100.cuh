@@ -1046,9 +1046,13 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       ok = ptx::mbar_spin_warp(&p_empty[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag);
       if (!ok) break;
       ptx::tc_fence_after();
-      const bool any = l_row != 0.f;                 // (a sum that is not a number stays one)
-      const float inv = any ? 1.f / l_row : 0.f;
-      const float total = any ? l_row * ex2(m_ref - m_true) : 0.f;     // relative to the row's maximum
+      // A row that sees no key here leaves nothing.  One whose scores here are all minus infinity has the sum 0: as a result it
+      // is no number (0 / 0); as a partial it has the sum 1 beside its maximum, so that it weighs nothing beside others, and
+      // O as it is (0 x infinity of a value is NaN in the value's column).  A sum that is not a number stays none.
+      const bool any = max(j.lo, j.key0 + first * kSpaKeys) < vis;
+      const bool low = slot >= 0 && l_row == 0.f;
+      const float inv = any ? (low ? 1.f : 1.f / l_row) : 0.f;
+      const float total = any ? (low ? 1.f : l_row * ex2(m_ref - m_true)) : 0.f;     // relative to the row's maximum
       const int32_t col0 = g * 256 + half * 128;     // this lane's columns
       if (slot >= 0) {
         float* o_row = a.p.part_o + ((int64_t)slot * 64 + col0 / 8) * (kSpaRows * 8) + trow * 8;

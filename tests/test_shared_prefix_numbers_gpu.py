@@ -37,3 +37,43 @@ def test_a_query_that_is_not_a_number_spoils_its_row_at_any_length(kind, bad, to
     first = rows_of(s["table"], 1, torch.tensor([0], device="cuda"), 64, s["cache"].shape[0])
     s["cache"].view(-1, 512)[first, 100] = 1.0          # (infinite queries: a score is +inf)
     _one_bad_row(s, bad, kind)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("tokens", [1, 2])
+@pytest.mark.parametrize("length", [3, 100, 129, 1000, 20000])
+def test_scores_of_minus_infinity_alone_are_no_number(kind, tokens, length):
+    """Every key's feature 100 is negative, the query's is infinite: 0 / 0, not a row that sees nothing."""
+    s = make(length, "BSND", [tokens] * 3, [length + 3, length, length + 40], 16, 64, 0)
+    s["cache"][..., 100] = -s["cache"][..., 100].abs() - 1
+    _one_bad_row(s, float("inf"), kind)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf")])
+def test_an_infinite_key_that_weighs_nothing_shows_in_its_column(kind, bad):
+    """Packed rows with one key of their own, whose score is -inf for some heads: 0 x infinity in the column of the value."""
+    lens = [641 + (i % 3) for i in range(70)]
+    hit = [b for b in (0, 33, 69)]
+    assert all(lens[b] == 641 for b in hit)
+    s = make(50, "BSND", [1] * 70, lens, 8, 64, 640)
+    want, room = _want(s)
+    without = reference(s["q"][:, 0], s["qr"][:, 0], s["cache"], s["rope"], s["table"], [1] * 70, [640] * 70, s["starts"], 1 / 24, 0)
+    for b in hit:
+        row = rows_of(s["table"], b, torch.tensor([640], device="cuda"), 64, s["cache"].shape[0])
+        s["cache"].view(-1, 512)[row, 77] = bad
+    with kernel(kind):
+        got = [g.reshape(w.shape) for g, w in zip(call(s), want)]
+    others = torch.ones(70, dtype=torch.bool, device="cuda")
+    others[hit] = False
+    check([g[others] for g in got], [w[others] for w in want], [r[others] for r in room], kind)
+    low = torch.stack([s["q"][b, 0, :, 77].float() * bad < 0 for b in hit])       # heads whose score is -inf
+    assert low.any() and not low.all()
+    assert torch.isnan(got[0][hit][~low]).all() and torch.isnan(got[1][hit][~low]).all() and torch.isnan(got[2][hit][~low]).all()
+    o = got[0][hit][low]
+    assert torch.isnan(o[:, 77]).all()
+    keep = torch.arange(512, device="cuda") != 77
+    diff = (o[:, keep].double() - without[0][0][hit][low][:, keep]).abs()
+    assert (diff <= without[1][0][hit][low][:, keep]).all()
+    for k in (1, 2):
+        assert ((got[k][hit][low].double() - without[0][k][hit][low]).abs() <= without[1][k][hit][low]).all()
