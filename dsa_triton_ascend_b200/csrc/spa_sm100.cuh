@@ -164,6 +164,10 @@ struct SpaSeq {
   int32_t vis0;                  // positions that its first token sees (may be negative)
   bool packed;
 };
+// Few enough rows, and some (s.packed: and the whole prefix seen by all of them)
+__device__ __forceinline__ bool spa_may_pack(const SpaDev& p, const SpaSeq& s) {
+  return s.act_q > 0 && (int64_t)s.act_q * p.n1 <= p.pack_rows;
+}
 __device__ __forceinline__ SpaSeq spa_seq(const SpaDev& p, int32_t b, int32_t prefix) {
   SpaSeq s;
   int32_t act_q;
@@ -187,8 +191,7 @@ __device__ __forceinline__ SpaSeq spa_seq(const SpaDev& p, int32_t b, int32_t pr
   s.act_k = max(0, min(act_k, p.seq.s2));
   // (the mask counts with the lengths as they were given)
   s.vis0 = p.seq.sparse_mode == 3 ? (int32_t)max((int64_t)-0x40000000, (int64_t)act_k - act_q + 1) : s.act_k;
-  s.packed = prefix >= kSpaPackKeys && s.act_q > 0 && (int64_t)s.act_q * p.n1 <= p.pack_rows && s.act_k >= prefix &&
-             s.vis0 >= prefix;
+  s.packed = prefix >= kSpaPackKeys && spa_may_pack(p, s) && s.act_k >= prefix && s.vis0 >= prefix;
   return s;
 }
 // First place of a sequence's row tiles in the list (behind the prefix tiles).
@@ -215,12 +218,15 @@ __device__ __noinline__ void spa_plan(const SpaDev& p, SpaPlanSmem& sm, int32_t 
   auto& place_s = sm.place_s;
   const int nt = blockDim.x, warps = nt >> 5;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // the longest sequence (the first of them) lends its pages for the prefix
+  // Of the sequences that may be packed, the one whose first token sees most (the first of them) lends its pages for the prefix.
+  // Others may have lengths and pages of before (a batch's idle slots, without query tokens), or see less than their length.
   int32_t prefix = 0, ref = 0;
   if (p.pack_rows > 0) {
     unsigned long long best = 0;
     for (int32_t b = tid; b < p.seq.batch; b += nt) {
-      const int32_t k = max(0, min(p.seq.seq_k[b], p.seq.s2));
+      const SpaSeq s = spa_seq(p, b, 0);
+      if (!spa_may_pack(p, s)) continue;
+      const int32_t k = max(0, min(s.act_k, s.vis0));
       best = max(best, ((unsigned long long)(uint32_t)k << 32) | (uint32_t)(0x7FFFFFFF - b));
     }
     const int32_t asked = p.prefix_device ? *p.prefix_device : p.prefix;

@@ -46,10 +46,11 @@ def shared_prefix_attention(
         actual_seq_lengths_query: [B] int32 / list / None (S1 each); cumulative, and required, for TND
         actual_seq_lengths_kv: [B] int32 / list: cached keys of each sequence, the prefix counted
         query_rope / key_rope: [..., 64], required
-        shared_prefix_length: how many first positions hold the same tokens in every sequence, an int or a
+        shared_prefix_length: how many first positions hold the same tokens in every sequence with query tokens, an int or a
             one-element int32 CUDA tensor (read when the call runs, so that a captured graph follows it).  They may be read
-            through any sequence's pages, so that they have to hold the same keys wherever a sequence has pages of its
-            own for them.  Sequences that do not see the whole prefix are computed from their own pages.  0: nothing is shared
+            through the pages of any such sequence that sees them all, so that the table has to lead each of them to the same
+            keys.  Sequences that do not see the whole prefix are computed from their own pages; sequences without
+            query tokens take no part, whatever their lengths and pages.  0: nothing is shared
         sparse_mode: 0 full / 3 rightDownCausal
         return_softmax_lse: also return the softmax statistics (zeros otherwise)
         block_size: paged block length (defaults to key.shape[1])

@@ -388,8 +388,10 @@ int dsa_latent_append(const DsaAppendParams* p, void* stream);
  *
  *   out[t, h] = sum_p softmax_p(scale * (query[t, h] . key[p] + query_rope[t, h] . key_rope[p])) key[p]
  * over the positions p < visible(t) of the token's sequence: seq_k (mode 0) or seq_k - seq_q + position + 1 (mode 3).
- * seq_k counts the prefix.  The first `prefix` positions of every sequence hold the same keys (the caller's promise):
- * they may be read through any sequence's row of the block table.  prefix_device, if not NULL, is read in place of
+ * seq_k counts the prefix.  The first `prefix` positions of every sequence with query tokens hold the same keys (the
+ * caller's promise): they may be read through the row of the block table of any such sequence that sees them all, so that
+ * each of these rows has to lead to them.  Sequences without query tokens take no part: their lengths and rows may be
+ * of before.  prefix_device, if not NULL, is read in place of
  * `prefix` when the call runs.  A length past a sequence's own is no error: a sequence that does not see the whole prefix is
  * computed from its own pages.  prefix = 0: plain attention over the paged cache.  Blocks that are absent (-1) or beyond the
  * cache inside a valid length read as zero keys that take part.  Rows without a visible key, padding rows and rows

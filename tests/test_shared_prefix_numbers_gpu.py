@@ -1,9 +1,9 @@
-"""shared_prefix_attention where numbers end: values that are not finite."""
+"""shared_prefix_attention where numbers end: values that are not finite, sequences that take no part."""
 import pytest
 import torch
 
 from tests.latent_ref import rows_of
-from tests.test_shared_prefix_gpu import KERNELS, call, check, kernel, make, reference
+from tests.test_shared_prefix_gpu import KERNELS, call, check, kernel, make, reference, verify
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,36 @@ def test_an_infinite_key_that_weighs_nothing_shows_in_its_column(kind, bad):
     assert (diff <= without[1][0][hit][low][:, keep]).all()
     for k in (1, 2):
         assert ((got[k][hit][low].double() - without[0][k][hit][low]).abs() <= without[1][k][hit][low]).all()
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("layout", ["BSND", "TND"])
+@pytest.mark.parametrize("stale", [-1, 0, 2**31 - 1])
+def test_sequences_without_query_tokens_do_not_lend_the_prefix(kind, layout, stale):
+    """Idle slots of a batch with lengths and table rows of before: the longest sequences, and their pages hold something else."""
+    q_lens = [1] * 75
+    kv = [700 + i % 50 for i in range(75)]
+    s = make(51, layout, q_lens, kv, 8, 64, 640)
+    blocks = s["cache"].shape[0]
+    for b in (0, 20, 74):
+        kv[b] = 800
+        s["table"][b] = stale if stale else blocks - 1
+    if layout == "BSND":
+        for b in (0, 20, 74):
+            q_lens[b] = 0
+    else:
+        for b in (0, 20, 74):
+            q_lens[b] = 0
+        ends = torch.tensor(q_lens).cumsum(0).tolist()
+        s["starts"], s["seq_q"] = [0] + ends[:-1], ends
+        s["q"], s["qr"] = s["q"][:ends[-1]].contiguous(), s["qr"][:ends[-1]].contiguous()
+    verify(s, kind)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+def test_a_longer_sequence_of_many_tokens_beside_packed_ones(kind):
+    """What is promised past the shorter sequences' ends: the packed ones meet as much as they see."""
+    q_lens = [2] * 75 + [60]
+    s = make(52, "TND", q_lens, [700 + i % 3 for i in range(75)] + [1500], 8, 64, 704)
+    for prefix in (640, 701, 704, 1400):
+        verify(s, kind, prefix=prefix)
