@@ -19,8 +19,9 @@
 // split along the value columns: CTA c loads all 128 keys x columns {c 128 .., 256 + c 128 ..}).  Q (72 KB a CTA), a tile of K
 // and three quarters of one of V fill the shared memory; M = 256 would need 144 KB of Q, and O of 128 rows all of tensor memory.
 // Tensor memory: lanes 0..63 hold a CTA's rows with the first half of N, lanes 64..127 the same rows with the second: O 256
-// columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off, so that a score is too small by 5e-7
-// of itself after 36 steps and a sum of exponentials too large by 2e-6; as two sums of 20 and 16 steps by half.)
+// columns, S 2 buffers x 2 partial sums x 64.  (The tensor cores cut the running sum off: of normally distributed queries and
+// keys a row's maximum is too small by 5e-7 of itself after 36 steps and its sum of exponentials too large by 2e-6; as two sums
+// of 20 and 16 steps by half.)
 //
 // Data movement.  Pages are whole in the cache, so that keys come with tiled TMA, as many per box (64, 32, 16, 8) as divide the
 // page size, else with gather4, four rows each.  Absent pages are read at a row past the tensor, which gives zeros without
@@ -99,10 +100,6 @@ constexpr uint32_t kSpaOffBar = kSpaOffX + 2048;
 constexpr uint32_t kSpaSmemBytes = kSpaOffBar + 512;
 static_assert(kSpaSmemBytes <= 232448, "shared memory");
 constexpr uint32_t kSpaTmO = 0, kSpaTmS = 256;
-// What the tensor cores cut off a score, in parts of it: the mean over the rows' maxima of products with 128 to 8000 keys, the same
-// at any scale of queries and keys (bf16 2.3 - 2.9e-7, fp16 3.2 - 3.8e-7).  The scale makes up for it: what is left is 1e-7 in
-// a maximum (root mean square; 2.5 and 3.5e-7 without) and 5.5 and 7.6e-7 in a sum over 8000 keys (1.0 and 1.4e-6 without).
-constexpr double kSpaCutBf16 = 2.5e-7, kSpaCutFp16 = 3.5e-7;
 constexpr float kSpaGuard = 8.f;     // log2 units that a score may exceed the reference by
 
 // One row tile against positions lo .. hi - 1, in tiles of 128 keys that start at key0.
@@ -1371,7 +1368,7 @@ inline int spa_sm100_launch(const DsaSpaParams* p, const SfaDev& dense, int32_t*
   d.out = p->out; d.softmax_max = p->softmax_max; d.softmax_sum = p->softmax_sum; d.return_lse = p->return_lse != 0;
   a.idesc_qk = ptx::idesc_f16(bf16 ? 1u : 0u, 128, kSpaKeys, 0, 0);
   a.idesc_pv = ptx::idesc_f16(bf16 ? 1u : 0u, 128, 256, 0, 1);
-  a.scale_log2 = (float)((double)p->scale * 1.4426950408889634 * (1.0 + (bf16 ? kSpaCutBf16 : kSpaCutFp16)));
+  a.scale_log2 = (float)((double)p->scale * 1.4426950408889634);
   a.is_bf16 = bf16 ? 1 : 0;
   a.key_rows = (int32_t)p->key_rows;
   a.blocks = (int32_t)(p->key_rows / p->block_size);

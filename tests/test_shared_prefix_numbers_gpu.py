@@ -1,4 +1,4 @@
-"""shared_prefix_attention where numbers end: values that are not finite, sequences that take no part."""
+"""shared_prefix_attention where numbers end: values that are not finite, exact scores, sequences that take no part."""
 import pytest
 import torch
 
@@ -110,3 +110,26 @@ def test_a_longer_sequence_of_many_tokens_beside_packed_ones(kind):
     s = make(52, "TND", q_lens, [700 + i % 3 for i in range(75)] + [1500], 8, 64, 704)
     for prefix in (640, 701, 704, 1400):
         verify(s, kind, prefix=prefix)
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_exact_scores_keep_their_maximum(kind, dtype):
+    """Queries with one feature: a score is one product, exact in 32 bits, and so is its product with a power of two.  What is left
+    of a maximum's error: the score in units of log2 and its way back are rounded once each (2^-24), and the two constants
+    are the nearest 32-bit numbers to log2 e and ln 2 (off by 1.4e-8 and 0.3e-8): below 2.5 x 2^-24."""
+    s = make(53, "BSND", [1] * 40, [900 + 3 * i for i in range(40)], 16, 64, 0, dtype)
+    s["q"].zero_()
+    s["qr"].zero_()
+    for h in range(16):
+        s["q"][:, 0, h, 32 * h + 5] = 1.5 + h / 8
+    flat = s["q"][:, 0].double()
+    with kernel(kind):
+        out, top, total = call(s, scale=0.25)
+    worst = 0.0
+    for b, n in enumerate(s["kv_lens"]):
+        row = rows_of(s["table"], b, torch.arange(n, device="cuda"), 64, s["cache"].shape[0])
+        score = flat[b] @ s["cache"].view(-1, 512)[row].double().T * 0.25
+        m = score.amax(1)
+        worst = max(worst, float(((top[b, 0, 0].double() - m).abs() / m.abs()).max()))
+    assert worst <= 2.5 * 2.0**-24, worst * 2**24
