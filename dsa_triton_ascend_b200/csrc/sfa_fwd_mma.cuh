@@ -7,6 +7,8 @@
 // (mma.sync m16n8k16, fp32 accumulation), the softmax in fp32 on the CUDA cores.
 #pragma once
 
+#include <type_traits>
+
 #include "dsa_common.cuh"
 #include "mma_sync.cuh"
 
@@ -72,6 +74,10 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
   const int g = lane >> 2, c4 = lane & 3;
   const RowInfo ri = row_info(p.seq, row);
   const bool row_active = kDense ? ri.visible > 0 : ri.pos < ri.act_q && ri.threshold > 0 && ri.act_k > 0;
+
+  // Dense rows may have many more keys than a selection: in fp16 their online probabilities are stored times 2^15 (the largest is
+  // 2^15), so that a long tail 10 to 27 nats below the maximum keeps its weight (the smallest number of the type is 2^-24).
+  constexpr float lift = kDense && std::is_same<T, __half>::value ? 32768.f : 1.f;
 
   // output accumulator: heads g and g + 8, d / 64 column tiles of 8 per warp (warp w: columns
   // (d / 8) w .. (d / 8) (w + 1) - 1), in the mma accumulator layout
@@ -211,7 +217,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
         float sum = pv;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        pt[h * PK + lane] = from_f32<T>(pv);
+        pt[h * PK + lane] = from_f32<T>(pv * lift);
         __syncwarp();
         if (lane == 0) {
           const float a = m_old == -INFINITY ? 0.f : expf(m_old - m_safe);
@@ -255,7 +261,7 @@ __device__ __forceinline__ void sfa_fwd_mma_row(const SfaDev& p, int32_t row, in
       if (h0 + h >= p.n1) continue;
       const float l = l_s[h];
       // (dense, l = 0: the accumulator is zero or NaN, and its product with infinity is NaN)
-      const float inv = two_pass ? 1.f : (kDense || l > 0.f ? 1.f / l : 0.f);
+      const float inv = two_pass ? 1.f : (kDense || l > 0.f ? 1.f / (l * lift) : 0.f);
       T* o = outp + (int64_t)h * p.d;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {

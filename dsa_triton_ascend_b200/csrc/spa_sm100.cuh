@@ -31,8 +31,8 @@
 // of 32 keys x 256 columns, refilled unit by unit; P has two buffers.
 //
 // Softmax.  Eight warps take every tile together: the four threads of a row (two halves of N x two groups of 32 keys) exchange
-// their maxima through shared memory.  P is relative to a running reference that follows the maximum only when it is
-// exceeded by more than 2^8: then O is rescaled in tensor memory (P <= 2^8 fits both types, the sums are fp32).  P is rounded to
+// their maxima through shared memory.  P is relative to a running reference that follows the maximum only when that has risen
+// by more than 2^8: then O is rescaled in tensor memory (P <= 2^8 in bf16, 2^15 in fp16; the sums are fp32).  P is rounded to
 // the io dtype, the operand type of the second product; its sum is that of the unrounded values.
 // Rows of one tile may see different numbers of keys (causal tokens of one sequence).  A hidden key has P = 0, and 0 x infinity
 // would be NaN: a hidden key whose score is not finite (every non-finite latent makes it so, for every row) marks the
@@ -100,7 +100,11 @@ constexpr uint32_t kSpaOffBar = kSpaOffX + 2048;
 constexpr uint32_t kSpaSmemBytes = kSpaOffBar + 512;
 static_assert(kSpaSmemBytes <= 232448, "shared memory");
 constexpr uint32_t kSpaTmO = 0, kSpaTmS = 256;
-constexpr float kSpaGuard = 8.f;     // log2 units that a score may exceed the reference by
+constexpr float kSpaGuard = 8.f;     // log2 units that the maximum may rise by before the reference follows
+// log2 units that the reference lies below the maximum that it was taken from, in fp16: P reaches from 2^15 at most down to the
+// type's smallest numbers, 21 nats below the maximum (without it 17, and half a step's accuracy ends 10 nats below: 4000 keys
+// 14 nats below a first one weighed 3 % too much or too little, and nothing 18 nats below).
+constexpr float kSpaLiftFp16 = 7.f;
 
 // One row tile against positions lo .. hi - 1, in tiles of 128 keys that start at key0.
 struct SpaJob {
@@ -912,6 +916,7 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint32_t s_empty_lead0 = ptx::map_to_rank(&s_empty[0], 0), s_empty_lead1 = ptx::map_to_rank(&s_empty[1], 0);
     const uint32_t p_full_lead = ptx::map_to_rank(&p_full[0], 0), o_free_lead = ptx::map_to_rank(o_free, 0);
     uint64_t* xb = &x_bar[quarter & 1];
+    const float lift = a.is_bf16 ? 0.f : kSpaLiftFp16;
     uint32_t n = 0, n_x = 0;
     bool ok = true;
     auto signal_lead = [&](uint64_t* local, uint32_t remote, bool publish) {
@@ -987,10 +992,12 @@ spa_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (!ok) break;
         const float mx = fmaxf(fmaxf(all.x, all.y), fmaxf(all.z, all.w));
         m_true = fmaxf(m_true, mx);
-        // the reference follows the maximum where it is exceeded by more than the guard (or where the row had none yet)
-        const bool raise = mx > m_ref + kSpaGuard || (m_ref == -INFINITY && mx > -INFINITY);
+        // The reference follows the maximum where that has risen by more than the guard (or where the row had none yet: the
+        // difference is infinite).  A difference of neighbours is exact; the reference plus the guard would be rounded, for
+        // scores of millions by more than what fp16 has left above P.
+        const bool raise = mx - m_ref > kSpaGuard + lift;
         if (__any_sync(0xffffffffu, raise)) {
-          const float m_new = raise ? mx : m_ref;
+          const float m_new = raise ? mx - lift : m_ref;
           const float f = raise ? (m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new)) : 1.f;
           l *= f;
           m_ref = m_new;

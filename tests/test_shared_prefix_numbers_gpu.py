@@ -1,4 +1,5 @@
-"""shared_prefix_attention where numbers end: values that are not finite, exact scores, sequences that take no part."""
+"""shared_prefix_attention where numbers end: queries, keys and scores that are not finite, exact scores, weights that fp16 hardly
+holds, sequences that take no part."""
 import pytest
 import torch
 
@@ -133,3 +134,56 @@ def test_exact_scores_keep_their_maximum(kind, dtype):
         m = score.amax(1)
         worst = max(worst, float(((top[b, 0, 0].double() - m).abs() / m.abs()).max()))
     assert worst <= 2.5 * 2.0**-24, worst * 2**24
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("below", [12.0, 14.0, 18.0])
+def test_a_long_tail_under_one_dominant_key_in_fp16(kind, below):
+    """4000 keys some nats below the first, which is zero as a value: the output is what the tail weighs.  P has to hold the
+    tail's weights at half a step of fp16, or of its smallest numbers 2^7 below the largest of P: 2^-25 x 2^-7 a key."""
+    n, B, H = 4000, 80, 128
+    g = torch.Generator(device="cuda").manual_seed(54)
+    table = torch.arange(63, device="cuda", dtype=torch.int32).repeat(B, 1)
+    cache = (8 + torch.randn(63, 64, 1, 512, generator=g, device="cuda")).half()
+    rope = torch.zeros(63, 64, 1, 64, device="cuda", dtype=torch.float16)
+    rope.view(-1, 64)[:, 0] = -below - torch.randint(0, 64, (63 * 64,), generator=g, device="cuda") / 256
+    cache.view(-1, 512)[0], rope.view(-1, 64)[0] = 0.0, 0.0
+    q, qr = torch.zeros(B, 1, H, 512, device="cuda").half(), torch.zeros(B, 1, H, 64, device="cuda").half()
+    qr[..., 0] = 1.0
+    s = dict(q=q, qr=qr, cache=cache, rope=rope, table=table, q_lens=[1] * B, kv_lens=[n] * B, starts=list(range(B)), seq_q=[1] * B,
+             layout="BSND", prefix=0)
+    with kernel(kind):
+        out = call(s, scale=1.0)[0].view(B * H, 512).double()
+    score, v = rope.view(-1, 64)[:n, 0].double(), cache.view(-1, 512)[:n].double()
+    e = torch.exp(score)
+    want = (e[:, None] * v).sum(0) / e.sum()
+    eps = torch.finfo(torch.float16).eps
+    # scores are exact up to the two roundings of their product with the scale, at most 20 x 2^-23; 32-bit sums as elsewhere
+    rel = eps / 2 + 20 * 2.0**-23 + (n / 16 + 64) * 2.0**-23
+    room = 1.05 * ((rel + eps / 2) * want + 2.0**-32 * v.sum(0) / e.sum()) + 2.0**-25
+    off = (out - want).abs() / room
+    assert off.max() <= 1, float(off.max())
+
+
+@pytest.mark.parametrize("kind", KERNELS)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scores_whose_steps_are_as_large_as_the_guard(kind, dtype):
+    """Scores around 4e7, where 32-bit numbers are 4 apart, that climb by 0 to 16 from tile to tile: outputs stay between the
+    smallest and the largest value (a weight past the type's largest number would be infinite)."""
+    n, B, H = 4000, 80, 128
+    g = torch.Generator(device="cuda").manual_seed(55)
+    dt = {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype]
+    table = torch.arange(16 * 63, device="cuda", dtype=torch.int32).view(16, 63).repeat(5, 1)
+    cache = torch.rand(16 * 63, 64, 1, 512, generator=g, device="cuda").to(dt)
+    rope = torch.zeros(16, 63 * 64, 64, device="cuda", dtype=dt)
+    climb = (4 * torch.randint(0, 5, (16, 32), generator=g, device="cuda")).cumsum(1).repeat_interleave(128, 1)[:, :63 * 64]
+    rope[..., 0] = 1220.0
+    rope[..., 1], rope[..., 2] = climb // 128, climb % 128           # (exact in either type)
+    q, qr = torch.zeros(B, 1, H, 512, device="cuda").to(dt), torch.zeros(B, 1, H, 64, device="cuda").to(dt)
+    qr[..., 0], qr[..., 1], qr[..., 2] = 32768.0, 128.0, 1.0
+    s = dict(q=q, qr=qr, cache=cache, rope=rope.view(16 * 63, 64, 1, 64), table=table, q_lens=[1] * B, kv_lens=[n] * B,
+             starts=list(range(B)), seq_q=[1] * B, layout="BSND", prefix=0)
+    with kernel(kind):
+        out, top, total = call(s, scale=1.0)
+    assert torch.isfinite(out).all() and torch.isfinite(top).all() and torch.isfinite(total).all()
+    assert (out >= 0).all() and (out <= 1 + 2.0**-7).all() and (total >= 1 - 2.0**-10).all()
