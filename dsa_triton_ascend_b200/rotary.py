@@ -64,11 +64,11 @@ def _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sec
     axes, sections = section_sizes(axis_sections, pairs)
     positions = check_positions(positions, tokens, axis_sections)
     one_device(x, positions, inv_freq)
+    if batch == 0 or s1 == 0 or n == 0:     # (contiguous whatever its strides are)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     if stride_d != 1:
         return _rotate(x.contiguous(), positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    if batch == 0 or s1 == 0 or n == 0:
-        return out
     p = _cabi.DsaRopeParams(
         _STRUCT_SIZE, inverse, x.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), out.data_ptr(), stride_b, stride_s,
         stride_n, code, positions.dtype is torch.int64, batch, s1, n, D, pairs, rotary_offset, bool(interleaved), axes, sections)
