@@ -78,6 +78,26 @@ def _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sec
     return out
 
 
+class _Rotation(torch.autograd.Function):
+    """The rotation for autograd: linear in x, and its transpose is the rotation by the opposite angles."""
+
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = (layout, interleaved, rotary_offset, None if axis_sections is None else tuple(axis_sections), not inverse)
+        return _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, "x")
+
+    @staticmethod
+    def backward(ctx, d_out):
+        return (_recorded(d_out, *ctx.saved_tensors, *ctx.how, "d_out"), *[None] * 7)
+
+
+def _recorded(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what):
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotation.apply(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse)
+    return _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, inverse, what)
+
+
 def rotary_embedding(x, positions, inv_freq, layout: str = "BSND", interleaved: bool = True, rotary_offset: int = 0,
                      axis_sections=None):
     """Rotate features of queries or keys by their tokens' positions.
@@ -94,16 +114,17 @@ def rotary_embedding(x, positions, inv_freq, layout: str = "BSND", interleaved: 
         axis_sections: pairs per position axis (time, height, width, ...), in order, up to four axes; None: one axis
 
     Returns: a new contiguous tensor of x's shape and dtype.  Angles are taken in 64 bits, sine, cosine and the rotation
-    in 32.  Nothing is recorded for autograd; the gradient is `rotary_embedding_grad`.
+    in 32.  Autograd records the call where x requires a gradient; without it the gradient is `rotary_embedding_grad`.
+    Positions and frequencies are not differentiated, and may not change before the backward pass.
     """
-    return _rotate(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, False, "x")
+    return _recorded(x, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, False, "x")
 
 
 def rotary_embedding_grad(d_out, positions, inv_freq, layout: str = "BSND", interleaved: bool = True,
                           rotary_offset: int = 0, axis_sections=None):
     """Gradient of `rotary_embedding` with respect to x, given the gradient of its result: the rotation by the
-    opposite angles.  Arguments as there; positions and frequencies are not differentiated."""
-    return _rotate(d_out, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, True, "d_out")
+    opposite angles.  Arguments as there."""
+    return _recorded(d_out, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, True, "d_out")
 
 
 class RotaryEmbedding(torch.nn.Module):
