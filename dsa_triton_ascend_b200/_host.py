@@ -70,6 +70,20 @@ def seq_tensor(lengths, device):
     raise ValueError("actual_seq_lengths must be None, a list/tuple or an int32 tensor")
 
 
+class KeepsFloat32(torch.nn.Module):
+    """Module whose float32 buffers stay float32, with their values, when the model around it is cast to another type; they
+    follow it to another device, and buffers of other types follow casts."""
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: t for name, t in self._buffers.items() if t is not None and t.dtype is torch.float32}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            now = self._buffers[name]
+            if now.dtype is not torch.float32:
+                self._buffers[name] = t.to(now.device)
+        return self
+
+
 def max_len_from_cumulative(host, fallback):
     """Largest per-sequence length of a cumulative list (upper bound `fallback` when unknown)."""
     if not host:

@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import _cabi
-from ._host import current_stream, device_guard, dtype_code, int32_table, one_device, ptr, seq_tensor
+from ._host import KeepsFloat32, current_stream, device_guard, dtype_code, int32_table, one_device, ptr, seq_tensor
 from .rotary import check_inv_freq, check_positions, section_sizes
 
 _VALID_D = (128, 256, 512)
@@ -165,8 +165,8 @@ def latent_cache_append(
     return latent_cache, rope_cache, index_cache
 
 
-class LatentCacheAppend(torch.nn.Module):
-    """Attribute holder around latent_cache_append."""
+class LatentCacheAppend(KeepsFloat32):
+    """Attribute holder around latent_cache_append.  inv_freq and a float32 norm_weight stay float32 when the model is cast."""
 
     def __init__(self, inv_freq, layout="BSND", norm_weight=None, norm_eps=1e-6, interleaved=True, index_interleaved=False,
                  index_rotary_offset=0, axis_sections=None):

@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from . import _cabi
-from ._host import current_stream, device_guard, dtype_code, one_device
+from ._host import KeepsFloat32, current_stream, device_guard, dtype_code, one_device
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _STRUCT_SIZE = ctypes.sizeof(_cabi.DsaRopeParams)
@@ -127,8 +127,8 @@ def rotary_embedding_grad(d_out, positions, inv_freq, layout: str = "BSND", inte
     return _recorded(d_out, positions, inv_freq, layout, interleaved, rotary_offset, axis_sections, True, "d_out")
 
 
-class RotaryEmbedding(torch.nn.Module):
-    """Attribute holder around rotary_embedding."""
+class RotaryEmbedding(KeepsFloat32):
+    """Attribute holder around rotary_embedding.  inv_freq stays float32 when the model is cast."""
 
     def __init__(self, inv_freq, layout="BSND", interleaved=True, rotary_offset=0, axis_sections=None):
         super().__init__()
