@@ -57,7 +57,8 @@ def shared_prefix_attention(
 
     Returns:
         (attention_out, softmax_max, softmax_sum); statistics are fp32 [B,1,S1,N1] (BSND) or [1,T1,N1] (TND).  Rows that see
-        no key give zeros.  Serving only: paged caches are not differentiated.
+        no key give zeros; rows whose softmax is no number (a score that is NaN or +infinity, or none but -infinity) give NaN in all
+        three.  Serving only: paged caches are not differentiated.
     """
     if sparse_mode not in (0, 3):
         raise ValueError("Only sparse_mode 0 (full) / 3 (rightDownCausal) supported")

@@ -395,7 +395,8 @@ int dsa_latent_append(const DsaAppendParams* p, void* stream);
  * `prefix` when the call runs.  A length past a sequence's own is no error: a sequence that does not see the whole prefix is
  * computed from its own pages.  prefix = 0: plain attention over the paged cache.  Blocks that are absent (-1) or beyond the
  * cache inside a valid length read as zero keys that take part.  Rows without a visible key, padding rows and rows
- * behind the last sequence give zeros in all three outputs.
+ * behind the last sequence give zeros in all three outputs; a row whose softmax is no number (a score that is NaN or
+ * +infinity, or none but -infinity) gives NaN in all three.
  */
 typedef struct DsaSpaParams {
   uint32_t struct_size; /* sizeof(DsaSpaParams) */
